@@ -304,7 +304,8 @@ int jq_quantize_q4_0_device(void *stream, const float *d_w, void *d_wq, int64_t 
 /* *fault_out is non-zero after a kernel of this library gave up on a bounded wait on the current device
  * (1: a bulk copy or pipeline stage never completed; 2: the bands of an all-gather never arrived), or, in the
  * range-checked debug build, skipped an access that fell outside its buffer (3); the word keeps the highest
- * code.  The call then returns JQ_ERR_TIMEOUT, else JQ_OK.  The kernel has returned, its output is not
+ * code.  The call then returns JQ_ERR_TIMEOUT, else JQ_OK.  (4, with JQ_ERR_INVALID_ARG: a page table named a page
+ * that its cache does not have; see jq_kv_cache.h.)  The kernel has returned, its output is not
  * valid, and the device stays usable.  Synchronises the device.  `clear` != 0 resets the word. */
 int jq_device_fault(int clear, int *fault_out);
 

@@ -37,13 +37,16 @@ CUDA_SOURCES = [
     "mmq_gemm_sm100.cu",
     "mmq_gemm_tc_sm100.cu",
     "mmq_gemm_f16_sm100.cu",
+    "rope.cu",
+    "paged_attention.cu",
+    "kv_evict.cu",
     "jq_capi.cu",
     "ref_compat.cpp",
     "weights_io.cpp",
     "model_q4_0.cpp",
 ]
-HEADERS = ["jq_common.cuh", "tc_common.cuh", "gemm_f16_plan.h", os.path.join(INCLUDE_DIR, "jq_b200.h"), os.path.join(INCLUDE_DIR, "jq_weights_io.h"),
-           os.path.join(INCLUDE_DIR, "jq_model.h")]
+HEADERS = ["jq_common.cuh", "tc_common.cuh", "gemm_f16_plan.h", "kv_cache.cuh", "kv_index.h", os.path.join(INCLUDE_DIR, "jq_b200.h"),
+           os.path.join(INCLUDE_DIR, "jq_weights_io.h"), os.path.join(INCLUDE_DIR, "jq_model.h"), os.path.join(INCLUDE_DIR, "jq_kv_cache.h")]
 BINDINGS = {"q8_1_me": "q8_1_binding.cpp", "mm_q4_0_q8_1_me": "mm_q4_0_q8_1_binding.cpp"}
 
 NVCC_FLAGS = [*os.environ.get("JQ_EXTRA_NVCC_FLAGS", "").split(),

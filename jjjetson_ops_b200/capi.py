@@ -33,6 +33,9 @@ KERNEL_NAMES = {
     KERNEL_GEMM_F16: "gemm_f16",
 }
 
+FAULT_BAD_PAGE = 4
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
+
 Q4_BYTES = 18
 Q8_BYTES = 144
 
@@ -99,6 +102,16 @@ _SIGS = {
     "jq_weights_device_ptr": (_vp, [_vp]),
     "jq_linear_q4_0_host": (_ci, [_vp, _vp, _vp, _vp, _i64, _ci]),
     "jq_query_device_hw_info": (_ci, [_ci, _vp]),
+    # jq_kv_cache.h
+    "jq_rope_table": (_ci, [_i64, ctypes.c_double, _ci, ctypes.c_double, _i64, _vp, ctypes.POINTER(ctypes.c_float)]),
+    "jq_rope_table_from": (_ci, [_vp, _i64, _vp]),
+    "jq_rope_device": (_ci, [_vp] * 5 + [_i64] * 8 + [_ci, ctypes.c_float]),
+    "jq_rope_kv_append_device": (_ci, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _ci, ctypes.c_float]),
+    "jq_paged_attention_ws_bytes": (_sz, [_i64, _i64, _vp, _ci]),
+    "jq_paged_attention_q8_1_device": (_ci, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, ctypes.c_float, _i64, _vp, _vp, _ci, _ci,
+                                             _vp, _i64, _i64, _vp, _sz]),
+    "jq_kv_evict_max_len": (_i64, []),
+    "jq_kv_evict_device": (_ci, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64]),
 }
 for _name, (_res, _args) in _SIGS.items():
     _fn = getattr(_lib, _name)
@@ -251,6 +264,114 @@ def swiglu_q8_1(gate: torch.Tensor, up: torch.Tensor, mid: Optional[torch.Tensor
     return xq
 
 
+def rope_table(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original_length: int = 0,
+               device=None, frequencies=None):
+    """The table of ``rope`` and ``rope_append`` on ``device`` (one entry per pair, turns per position in fixed point) and the
+    factor of sine and cosine: ``(table, mscale)``.  ``scaling`` is a key of ``ROPE_SCALING``; ``frequencies`` (radians per
+    position of every pair) takes the place of ``base`` and ``scaling``.  Make it once."""
+    n = rotary_dim // 2
+    table, mscale = (ctypes.c_uint64 * max(n, 1))(), ctypes.c_float(1.0)
+    if frequencies is not None:
+        if len(frequencies) != n:
+            raise ValueError("%d frequencies where %d are expected" % (len(frequencies), n))
+        check(_lib.jq_rope_table_from((ctypes.c_double * max(n, 1))(*[float(f) for f in frequencies]), n, table))
+    else:
+        if scaling not in ROPE_SCALING:
+            raise ValueError("scaling must be one of %s" % ", ".join(sorted(ROPE_SCALING)))
+        check(_lib.jq_rope_table(rotary_dim, base, ROPE_SCALING[scaling], factor, original_length, table, ctypes.byref(mscale)))
+    as_int64 = (ctypes.c_int64 * max(n, 1)).from_buffer(table)
+    return torch.tensor(list(as_int64)[:n], dtype=torch.int64, device=device), float(mscale.value)
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interleaved: bool = False, mscale: float = 1.0,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions: ``x`` fp32 ``[T, H, D]`` (rows and heads may be strided), ``positions`` int32 ``[T]``.  The first
+    ``2 * len(table)`` elements of every head turn, in halves or ``interleaved`` pairs; ``out`` may be ``x``."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    rc = _calls.rope(x, out, positions, table, interleaved, mscale)
+    if rc:
+        check(rc)
+    return out
+
+
+def rope_append(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                page_table: torch.Tensor, index: torch.Tensor, seqs: Optional[torch.Tensor] = None,
+                q_out: Optional[torch.Tensor] = None, interleaved: bool = False, mscale: float = 1.0, k_scale: float = 1.0,
+                v_scale: float = 1.0) -> torch.Tensor:
+    """The fused projection's output ``qkv`` ``[T, (Hq + 2 Hkv) * D]`` -> rotated queries ``[T, Hq, D]`` (returned), rotated keys and
+    values in the paged cache.  ``k_cache`` and ``v_cache`` are ``[pages, slots, Hkv, D]`` (float16, bfloat16 or float8_e4m3fn, any
+    strides that are multiples of 16 bytes), ``page_table`` int32 ``[sequences, pages of one]``.  Row ``t`` becomes token
+    ``index[t]`` of sequence ``seqs[t]`` (default: ``t``); a negative sequence or index marks padding."""
+    if q_out is None:
+        D = k_cache.shape[3]
+        q_out = torch.empty((qkv.shape[0], max(0, qkv.shape[1] // max(D, 1) - 2 * k_cache.shape[2]), D), dtype=torch.float32, device=qkv.device)
+    rc = _calls.rope_append(qkv, q_out, positions, table, k_cache, v_cache, page_table, index, seqs, k_scale, v_scale, interleaved, mscale)
+    if rc:
+        check(rc)
+    return q_out
+
+
+def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor, weights: bool = False) -> torch.Tensor:
+    """Workspace of ``paged_attention_q8_1`` for queries, caches and tables of these shapes, whatever the lengths; ``weights``: for
+    calls that accumulate weights.  It serves call after call on one stream; calls that can overlap need one each."""
+    n = _calls.attention_ws_bytes(q, k_cache, page_table, weights)
+    if n == 0:
+        raise JqError(ERR_INVALID_ARG, last_error())
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    ws[: 4 * q.shape[0] * q.shape[1]].zero_()  # the counters
+    return ws
+
+
+def paged_attention_q8_1(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                         seqs: Optional[torch.Tensor] = None, scale: Optional[float] = None, window: int = 0, k_scale: float = 1.0,
+                         v_scale: float = 1.0, out: Optional[torch.Tensor] = None, want_q8: bool = True,
+                         order: int = ORDER_COL_KSUPER, s_mode: int = S_D_SUM_Q, xq: Optional[torch.Tensor] = None,
+                         weights: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Attention of one query token per row, ``q`` fp32 ``[T, Hq, D]``, over the first ``lens[t]`` tokens (the last ``window`` of them)
+    of sequence ``seqs[t]`` (default: ``t``) in the paged cache of ``rope_append``.  ``out`` receives the fp32 result; the returned
+    uint8 tensor holds the Q8_1 blocks of it (``None`` when ``want_q8`` is false).  ``scale`` defaults to ``1 / sqrt(D)``.  To
+    ``weights`` (fp32 ``[T, Hkv, tokens]``) is added what the step gave to each token.  Without ``ws``
+    (``paged_attention_workspace``) a workspace is made for the call."""
+    if want_q8 and xq is None:
+        xq = torch.empty(max(q8_1_bytes(q.shape[1] * q.shape[2], q.shape[0]), 16), dtype=torch.uint8, device=q.device)
+    if not want_q8:
+        xq = None
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if ws is None:
+        ws = paged_attention_workspace(q, k_cache, page_table, weights is not None)
+    rc = _calls.attention(q, k_cache, v_cache, page_table, lens, seqs, scale, window, k_scale, v_scale, out, xq, order, s_mode, weights, ws)
+    if rc:
+        check(rc)
+    return xq
+
+
+def kv_evict(weights: torch.Tensor, lens: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+             keep: int, recent: int = 0, sinks: int = 0, new_page_table: Optional[torch.Tensor] = None,
+             new_weights: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None,
+             kept: Optional[torch.Tensor] = None):
+    """Cuts every sequence of the cache down to ``keep`` tokens per key-value head: the first ``sinks``, the last ``recent`` and
+    those of the largest ``weights`` ``[sequences, Hkv, tokens]``, in their order.  They move to the pages of ``new_page_table``
+    (other pages of the same pool) or, by default, to the front of their own.  Returns ``(kept, new_lens)``: the tokens' former
+    indices ``[sequences, Hkv, keep]`` (-1 behind the last) and the new lengths.  ``new_weights`` (default: ``weights`` itself)
+    receives the kept tokens' weights, then zeros.  ``new_lens`` may be ``lens``."""
+    if kept is None:
+        kept = torch.empty((weights.shape[0], weights.shape[1], keep), dtype=torch.int32, device=weights.device)
+    if new_lens is None:
+        new_lens = torch.empty_like(lens)
+    rc = _calls.evict(weights, lens, k_cache, v_cache, page_table, new_page_table, keep, recent, sinks, kept, new_lens,
+                      weights if new_weights is None else new_weights)
+    if rc:
+        check(rc)
+    return kept, new_lens
+
+
+def kv_evict_max_len() -> int:
+    """The longest row of weights that ``kv_evict`` takes."""
+    return int(_lib.jq_kv_evict_max_len())
+
+
 NOALLOC_WS_BYTES = 4 << 20
 
 
@@ -363,11 +484,12 @@ def quantize_q4_0(w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.
 
 
 def device_fault(clear: bool = True) -> int:
-    """The device's fault word (0: no bounded wait has given up).  A non-zero word comes with status
-    JQ_ERR_TIMEOUT, which is reported through the return value here, not raised."""
+    """The device's fault word (0: no bounded wait has given up, no page table named a page that does not exist).  A
+    non-zero word comes with status JQ_ERR_TIMEOUT (``FAULT_BAD_PAGE``: JQ_ERR_INVALID_ARG), which is reported through
+    the return value here, not raised."""
     v = ctypes.c_int(0)
     rc = _lib.jq_device_fault(1 if clear else 0, ctypes.byref(v))
-    if rc not in (OK, ERR_TIMEOUT):
+    if rc not in (OK, ERR_TIMEOUT) and not (rc == ERR_INVALID_ARG and v.value == FAULT_BAD_PAGE):
         check(rc)
     return int(v.value)
 

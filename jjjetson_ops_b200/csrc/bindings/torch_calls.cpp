@@ -20,6 +20,7 @@
 #include <cstdint>
 
 #include "../../../include/jq_b200.h"
+#include "../../../include/jq_kv_cache.h"
 
 namespace {
 
@@ -30,6 +31,11 @@ decltype(&jq_linear_q4_0_device) f_linear = nullptr;
 decltype(&jq_linear_q4_0_multi_device) f_multi = nullptr;
 decltype(&jq_rms_norm_q8_1_device) f_rms_norm = nullptr;
 decltype(&jq_swiglu_q8_1_device) f_swiglu = nullptr;
+decltype(&jq_rope_device) f_rope = nullptr;
+decltype(&jq_rope_kv_append_device) f_rope_append = nullptr;
+decltype(&jq_paged_attention_ws_bytes) f_attention_ws_bytes = nullptr;
+decltype(&jq_paged_attention_q8_1_device) f_attention = nullptr;
+decltype(&jq_kv_evict_device) f_evict = nullptr;
 
 struct Binding {
     const char *name;
@@ -42,6 +48,11 @@ const Binding bindings[] = {
     {"jq_linear_q4_0_multi_device", reinterpret_cast<void **>(&f_multi)},
     {"jq_rms_norm_q8_1_device", reinterpret_cast<void **>(&f_rms_norm)},
     {"jq_swiglu_q8_1_device", reinterpret_cast<void **>(&f_swiglu)},
+    {"jq_rope_device", reinterpret_cast<void **>(&f_rope)},
+    {"jq_rope_kv_append_device", reinterpret_cast<void **>(&f_rope_append)},
+    {"jq_paged_attention_ws_bytes", reinterpret_cast<void **>(&f_attention_ws_bytes)},
+    {"jq_paged_attention_q8_1_device", reinterpret_cast<void **>(&f_attention)},
+    {"jq_kv_evict_device", reinterpret_cast<void **>(&f_evict)},
 };
 
 PyObject *bind(PyObject *, PyObject *addresses) {
@@ -64,7 +75,9 @@ struct Owned {
 };
 
 // ---- arguments -------------------------------------------------------------------------------------
-const char *dtype_text(at::ScalarType t) { return t == at::kFloat ? "torch.float32" : "torch.uint8"; }
+const char *dtype_text(at::ScalarType t) {
+    return t == at::kFloat ? "torch.float32" : t == at::kInt ? "torch.int32" : t == at::kLong ? "torch.int64" : "torch.uint8";
+}
 
 // The tensor behind `o` when it is a contiguous CUDA tensor of this type, else nullptr with ValueError set.
 const at::Tensor *tensor_arg(PyObject *o, at::ScalarType type, const char *name) {
@@ -290,6 +303,274 @@ PyObject *swiglu(PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// ---- the paged cache and what reads and writes it: strided tensors, all on one device, sizes checked against one another --------------
+// The tensor behind `o` when it is a CUDA tensor of this type with `dims` dimensions whose last one is contiguous, on the device of `like`
+// (when given), else nullptr with ValueError set.
+const at::Tensor *strided_arg(PyObject *o, at::ScalarType type, int64_t dims, const char *name, const at::Tensor *like) {
+    if (THPVariable_Check(o)) {
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (t.is_cuda() && t.scalar_type() == type && t.dim() == dims && (t.size(dims - 1) <= 1 || t.stride(dims - 1) == 1)) {
+            if (like == nullptr || t.get_device() == like->get_device()) return &t;
+            PyErr_Format(PyExc_ValueError, "%s is on another device than the other tensors", name);
+            return nullptr;
+        }
+    }
+    PyErr_Format(PyExc_ValueError, "%s must be a CUDA tensor of dtype %s with %d dimensions, the last one contiguous", name, dtype_text(type), (int)dims);
+    return nullptr;
+}
+bool size_is(int64_t got, int64_t want, const char *name, const char *what) {
+    if (got == want) return true;
+    PyErr_Format(PyExc_ValueError, "%s has %lld %s where %lld are expected", name, (long long)got, what, (long long)want);
+    return false;
+}
+// A contiguous vector of `n` int32 on the device of `like`; None where that is allowed.
+bool vector_arg(PyObject *o, int64_t n, const char *name, const at::Tensor &like, bool optional, const int32_t **out) {
+    *out = nullptr;
+    if (optional && o == Py_None) return true;
+    const at::Tensor *t = strided_arg(o, at::kInt, 1, name, &like);
+    if (t == nullptr || !size_is(t->size(0), n, name, "elements")) return false;
+    *out = static_cast<const int32_t *>(t->data_ptr());
+    return true;
+}
+bool double_arg(PyObject *o, double *out) {
+    *out = PyFloat_AsDouble(o);
+    return !(*out == -1.0 && PyErr_Occurred());
+}
+bool truth_arg(PyObject *o, int *out) {
+    *out = PyObject_IsTrue(o);
+    return *out >= 0;
+}
+
+// (k, v, page_table): k and v [pages, slot, head, element] of one type with the same sizes and strides.
+bool cache_arg(PyObject *ko, PyObject *vo, PyObject *to, const at::Tensor *like, jq_kv_cache *c, const at::Tensor **k_out) {
+    if (!THPVariable_Check(ko)) {
+        PyErr_SetString(PyExc_ValueError, "k_cache must be a tensor");
+        return false;
+    }
+    const at::ScalarType type = THPVariable_Unpack(ko).scalar_type();
+    if (type == at::kHalf)
+        c->type = JQ_KV_F16;
+    else if (type == at::kBFloat16)
+        c->type = JQ_KV_BF16;
+    else if (type == at::kFloat8_e4m3fn)
+        c->type = JQ_KV_E4M3;
+    else {
+        PyErr_SetString(PyExc_ValueError, "k_cache must have dtype torch.float16, torch.bfloat16 or torch.float8_e4m3fn");
+        return false;
+    }
+    const at::Tensor *k = nullptr, *v = nullptr;
+    for (PyObject *o : {ko, vo}) {
+        const char *name = o == ko && k == nullptr ? "k_cache" : "v_cache";
+        const at::Tensor *t = nullptr;
+        if (THPVariable_Check(o)) t = &THPVariable_Unpack(o);
+        if (t == nullptr || !t->is_cuda() || t->scalar_type() != type || t->dim() != 4 || t->stride(3) != 1) {
+            PyErr_Format(PyExc_ValueError, "%s must be a CUDA tensor [pages, slots, heads, elements] of the cache's dtype, the last dimension contiguous", name);
+            return false;
+        }
+        (k == nullptr ? k : v) = t;
+    }
+    const at::Tensor *table = strided_arg(to, at::kInt, 2, "page_table", k);
+    if (table == nullptr) return false;
+    if (v->get_device() != k->get_device() || (like != nullptr && like->get_device() != k->get_device())) {
+        PyErr_SetString(PyExc_ValueError, "the cache is on another device than the other tensors");
+        return false;
+    }
+    for (int i = 0; i < 4; ++i) {
+        if (k->size(i) != v->size(i) || k->stride(i) != v->stride(i)) {
+            PyErr_SetString(PyExc_ValueError, "k_cache and v_cache must have the same sizes and strides");
+            return false;
+        }
+    }
+    c->d_k = k->data_ptr();
+    c->d_v = v->data_ptr();
+    c->num_pages = k->size(0), c->page_size = k->size(1), c->num_kv_heads = k->size(2), c->head_dim = k->size(3);
+    c->stride_page = k->stride(0), c->stride_slot = k->stride(1), c->stride_head = k->stride(2);
+    c->k_scale = c->v_scale = 1.f;
+    c->d_page_table = static_cast<const int32_t *>(table->data_ptr());
+    c->num_seqs = table->size(0), c->max_pages = table->size(1);
+    c->table_stride = table->size(0) > 1 ? table->stride(0) : table->size(1);
+    *k_out = k;
+    return true;
+}
+
+// (x, out, positions, table, interleaved, mscale)
+PyObject *rope(PyObject *const *a, Py_ssize_t n) {
+    const int32_t *positions;
+    int interleaved;
+    double mscale;
+    if (!argument_count(n, 6)) return nullptr;
+    const at::Tensor *x = strided_arg(a[0], at::kFloat, 3, "x", nullptr);
+    if (x == nullptr) return nullptr;
+    const at::Tensor *out = strided_arg(a[1], at::kFloat, 3, "out", x), *table = strided_arg(a[3], at::kLong, 1, "table", x);
+    if (out == nullptr || table == nullptr || !vector_arg(a[2], x->size(0), "positions", *x, false, &positions) || !truth_arg(a[4], &interleaved) ||
+        !double_arg(a[5], &mscale))
+        return nullptr;
+    for (int i = 0; i < 3; ++i) {
+        if (!size_is(out->size(i), x->size(i), "out", "elements in a dimension")) return nullptr;
+    }
+    const float *xp = static_cast<const float *>(x->data_ptr());
+    float *yp = static_cast<float *>(out->data_ptr());
+    const uint64_t *tp = static_cast<const uint64_t *>(table->data_ptr());
+    const int64_t T = x->size(0), H = x->size(1), D = x->size(2), R = 2 * table->size(0);
+    const int64_t s[4] = {x->stride(0), x->stride(1), out->stride(0), out->stride(1)};
+    return status_of(*x, [&](void *st) { return f_rope(st, xp, yp, positions, tp, T, H, D, R, s[0], s[1], s[2], s[3], interleaved, (float)mscale); });
+}
+
+// (qkv, q_out, positions, table, k, v, page_table, index, seqs or None, k_scale, v_scale, interleaved, mscale)
+PyObject *rope_append(PyObject *const *a, Py_ssize_t n) {
+    const int32_t *positions, *index, *seqs;
+    int interleaved;
+    double mscale, k_scale, v_scale;
+    jq_kv_cache c = {};
+    const at::Tensor *k = nullptr;
+    if (!argument_count(n, 13)) return nullptr;
+    const at::Tensor *x = strided_arg(a[0], at::kFloat, 2, "qkv", nullptr);
+    if (x == nullptr) return nullptr;
+    const int64_t T = x->size(0);
+    const at::Tensor *q = strided_arg(a[1], at::kFloat, 3, "q_out", x), *table = strided_arg(a[3], at::kLong, 1, "table", x);
+    if (q == nullptr || table == nullptr || !cache_arg(a[4], a[5], a[6], x, &c, &k) || !vector_arg(a[2], T, "positions", *x, false, &positions) ||
+        !vector_arg(a[7], T, "index", *x, false, &index) || !vector_arg(a[8], T, "seqs", *x, true, &seqs) || !double_arg(a[9], &k_scale) ||
+        !double_arg(a[10], &v_scale) || !truth_arg(a[11], &interleaved) || !double_arg(a[12], &mscale))
+        return nullptr;
+    const int64_t H = q->size(1);
+    if (!size_is(q->size(0), T, "q_out", "rows") || !size_is(q->size(2), c.head_dim, "q_out", "elements in a head") ||
+        !size_is(x->size(1), (H + 2 * c.num_kv_heads) * c.head_dim, "qkv", "columns"))
+        return nullptr;
+    c.k_scale = (float)k_scale, c.v_scale = (float)v_scale;
+    const float *xp = static_cast<const float *>(x->data_ptr());
+    float *qp = static_cast<float *>(q->data_ptr());
+    const uint64_t *tp = static_cast<const uint64_t *>(table->data_ptr());
+    const int64_t R = 2 * table->size(0), s[3] = {x->stride(0), q->stride(0), q->stride(1)};
+    return status_of(*x, [&](void *st) {
+        return f_rope_append(st, xp, s[0], qp, s[1], s[2], positions, index, seqs, tp, R, T, H, &c, interleaved, (float)mscale);
+    });
+}
+
+// (q, k, page_table, weights) -> bytes; 0 after an error
+PyObject *attention_ws_bytes(PyObject *const *a, Py_ssize_t n) {
+    int weights;
+    jq_kv_cache c = {};
+    const at::Tensor *k = nullptr;
+    if (!argument_count(n, 4)) return nullptr;
+    const at::Tensor *q = strided_arg(a[0], at::kFloat, 3, "q", nullptr);
+    if (q == nullptr || !cache_arg(a[1], a[1], a[2], q, &c, &k) || !truth_arg(a[3], &weights)) return nullptr;
+    OnDevice device(*q);
+    const size_t bytes = f_attention_ws_bytes(q->size(0), q->size(1), &c, weights);
+    device.restore();
+    return PyLong_FromSize_t(bytes);
+}
+
+// (q, k, v, page_table, lens, seqs or None, scale, window, k_scale, v_scale, out or None, xq or None, order, s_mode, weights or None, ws)
+PyObject *attention(PyObject *const *a, Py_ssize_t n) {
+    const int32_t *lens, *seqs;
+    double scale, k_scale, v_scale;
+    int64_t window, order, s_mode, weights_stride = 0, weights_len = 0;
+    jq_kv_cache c = {};
+    const at::Tensor *k = nullptr;
+    if (!argument_count(n, 16)) return nullptr;
+    const at::Tensor *q = strided_arg(a[0], at::kFloat, 3, "q", nullptr);
+    if (q == nullptr) return nullptr;
+    const int64_t T = q->size(0), H = q->size(1);
+    if (!cache_arg(a[1], a[2], a[3], q, &c, &k) || !size_is(q->size(2), c.head_dim, "q", "elements in a head") ||
+        !vector_arg(a[4], T, "lens", *q, false, &lens) || !vector_arg(a[5], T, "seqs", *q, true, &seqs) || !double_arg(a[6], &scale) ||
+        !size_arg(a[7], &window) || !double_arg(a[8], &k_scale) || !double_arg(a[9], &v_scale) || !size_arg(a[12], &order) || !size_arg(a[13], &s_mode))
+        return nullptr;
+    c.k_scale = (float)k_scale, c.v_scale = (float)v_scale;
+    float *out = nullptr, *weights = nullptr;
+    void *xq = nullptr;
+    if (a[10] != Py_None) {
+        const at::Tensor *t = tensor_arg(a[10], at::kFloat, "out");
+        if (t == nullptr || !size_is(t->numel(), q->numel(), "out", "elements")) return nullptr;
+        if (t->get_device() != q->get_device()) {
+            PyErr_SetString(PyExc_ValueError, "out is on another device than the other tensors");
+            return nullptr;
+        }
+        out = static_cast<float *>(t->data_ptr());
+    }
+    if (a[11] != Py_None) {
+        const at::Tensor *t = tensor_arg(a[11], at::kByte, "xq");
+        if (t == nullptr) return nullptr;
+        if (t->numel() < T * ((H * c.head_dim + 127) / 128) * 144 || t->get_device() != q->get_device()) {
+            PyErr_SetString(PyExc_ValueError, "xq is too small for the Q8_1 blocks, or on another device");
+            return nullptr;
+        }
+        xq = t->data_ptr();
+    }
+    if (a[14] != Py_None) {
+        const at::Tensor *t = strided_arg(a[14], at::kFloat, 3, "weights", q);
+        if (t == nullptr || !size_is(t->size(0), T, "weights", "rows") || !size_is(t->size(1), c.num_kv_heads, "weights", "heads")) return nullptr;
+        weights_stride = c.num_kv_heads > 1 ? t->stride(1) : T > 1 ? t->stride(0) : t->size(2);
+        if ((T > 1 && c.num_kv_heads > 1 && t->stride(0) != weights_stride * c.num_kv_heads)) {
+            PyErr_SetString(PyExc_ValueError, "weights must have its rows and heads evenly spaced");
+            return nullptr;
+        }
+        weights_len = t->size(2);
+        weights = static_cast<float *>(t->data_ptr());
+    }
+    const at::Tensor *ws = tensor_arg(a[15], at::kByte, "ws");
+    if (ws == nullptr) return nullptr;
+    if (ws->get_device() != q->get_device()) {
+        PyErr_SetString(PyExc_ValueError, "ws is on another device than the other tensors");
+        return nullptr;
+    }
+    void *wp = ws->data_ptr();
+    const size_t ws_bytes = (size_t)ws->numel();
+    const float *qp = static_cast<const float *>(q->data_ptr());
+    const int64_t s[2] = {q->stride(0), q->stride(1)};
+    return status_of(*q, [&](void *st) {
+        return f_attention(st, qp, s[0], s[1], T, H, &c, lens, seqs, (float)scale, window, out, xq, (int)order, (int)s_mode, weights, weights_stride, weights_len,
+                           wp, ws_bytes);
+    });
+}
+
+// (weights, lens, k, v, page_table, new_page_table or None, keep, recent, sinks, kept, new_lens, new_weights)
+PyObject *evict(PyObject *const *a, Py_ssize_t n) {
+    const int32_t *lens, *new_lens, *new_table = nullptr;
+    int64_t keep, recent, sinks, new_pages = 0, new_stride = 0;
+    jq_kv_cache c = {};
+    const at::Tensor *k = nullptr;
+    if (!argument_count(n, 12)) return nullptr;
+    const at::Tensor *w = strided_arg(a[0], at::kFloat, 3, "weights", nullptr);
+    if (w == nullptr || !cache_arg(a[2], a[3], a[4], w, &c, &k)) return nullptr;
+    const int64_t B = c.num_seqs, H = c.num_kv_heads;
+    if (!vector_arg(a[1], B, "lens", *w, false, &lens) || !size_arg(a[6], &keep) || !size_arg(a[7], &recent) || !size_arg(a[8], &sinks) ||
+        !vector_arg(a[10], B, "new_lens", *w, false, &new_lens))
+        return nullptr;
+    const at::Tensor *nw = strided_arg(a[11], at::kFloat, 3, "new_weights", w), *kept = tensor_arg(a[9], at::kInt, "kept");
+    if (nw == nullptr || kept == nullptr) return nullptr;
+    if (kept->get_device() != w->get_device() || kept->numel() != B * H * keep) {
+        PyErr_SetString(PyExc_ValueError, "kept must have [sequences, heads, keep] elements on the device of the other tensors");
+        return nullptr;
+    }
+    int64_t stride[2];
+    const at::Tensor *both[2] = {w, nw};
+    for (int i = 0; i < 2; ++i) {
+        const char *name = i == 0 ? "weights" : "new_weights";
+        if (!size_is(both[i]->size(0), B, name, "rows") || !size_is(both[i]->size(1), H, name, "heads") || !size_is(both[i]->size(2), w->size(2), name, "tokens"))
+            return nullptr;
+        stride[i] = H > 1 ? both[i]->stride(1) : B > 1 ? both[i]->stride(0) : both[i]->size(2);
+        if (B > 1 && H > 1 && both[i]->stride(0) != stride[i] * H) {
+            PyErr_Format(PyExc_ValueError, "%s must have its rows and heads evenly spaced", name);
+            return nullptr;
+        }
+    }
+    if (a[5] != Py_None) {
+        const at::Tensor *t = strided_arg(a[5], at::kInt, 2, "new_page_table", w);
+        if (t == nullptr || !size_is(t->size(0), B, "new_page_table", "rows")) return nullptr;
+        new_table = static_cast<const int32_t *>(t->data_ptr());
+        new_pages = t->size(1);
+        new_stride = B > 1 ? t->stride(0) : t->size(1);
+    }
+    const float *wp = static_cast<const float *>(w->data_ptr());
+    float *nwp = static_cast<float *>(nw->data_ptr());
+    int32_t *kp = static_cast<int32_t *>(kept->data_ptr());
+    const int64_t S = w->size(2);
+    return status_of(*w, [&](void *st) {
+        return f_evict(st, &c, lens, wp, stride[0], S, keep, recent, sinks, new_table, new_pages, new_stride, kp, const_cast<int32_t *>(new_lens), nwp,
+                       stride[1]);
+    });
+}
+
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&entry<f>)), METH_FASTCALL
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, "Addresses of the library's functions, by name."},
@@ -299,6 +580,13 @@ PyMethodDef methods[] = {
     {"multi", FAST(multi), "(ws_list, N_list, outs, x, xq, ws, K, M, s_mode) -> status"},
     {"rms_norm", FAST(rms_norm), "(x, weight, epsilon, residual, normed, xq, order, s_mode) -> status"},
     {"swiglu", FAST(swiglu), "(gate, up, mid, xq, order, s_mode) -> status"},
+    {"rope", FAST(rope), "(x, out, positions, table, interleaved, mscale) -> status"},
+    {"rope_append", FAST(rope_append),
+     "(qkv, q_out, positions, table, k, v, page_table, index, seqs, k_scale, v_scale, interleaved, mscale) -> status"},
+    {"attention_ws_bytes", FAST(attention_ws_bytes), "(q, k, page_table, weights) -> bytes"},
+    {"attention", FAST(attention),
+     "(q, k, v, page_table, lens, seqs, scale, window, k_scale, v_scale, out, xq, order, s_mode, weights, ws) -> status"},
+    {"evict", FAST(evict), "(weights, lens, k, v, page_table, new_page_table, keep, recent, sinks, kept, new_lens, new_weights) -> status"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", "Native part of capi.py's tensor calls.", -1, methods};

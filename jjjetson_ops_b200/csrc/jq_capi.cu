@@ -771,6 +771,8 @@ int jq_device_fault(int clear, int *fault_out) {
         JQ_CUDA_TRY(cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice));
     }
     if (fault_out) *fault_out = v;
+    if (v == 4)
+        return set_error(JQ_ERR_INVALID_ARG, "a page table named a page that the cache does not have: its tokens were neither written nor attended to");
     if (v == 3)
         return set_error(JQ_ERR_TIMEOUT, "a range check of the debug build failed: an access outside its buffer was skipped");
     if (v != 0)

@@ -1,0 +1,47 @@
+// Where a token of a paged cache lies, as the kernels and the tests on the CPU compute it.  Plain C++.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define JQ_HOST_DEVICE __host__ __device__ __forceinline__
+#else
+#define JQ_HOST_DEVICE inline
+#endif
+
+namespace jq {
+
+// The indices of one cache (see jq_kv_cache); all sizes have been checked to fit.
+struct KvIndex {
+    const int32_t *table;
+    int64_t table_stride;
+    int64_t stride_page, stride_slot, stride_head;  // in elements
+    int32_t num_seqs, max_pages, num_pages, page_size;
+    int32_t page_shift;  // log2 of page_size where it is a power of two, else -1: a general division costs some 20 instructions
+};
+
+JQ_HOST_DEVICE uint32_t kv_page_of(const KvIndex &ix, uint32_t token) {
+    return ix.page_shift >= 0 ? token >> ix.page_shift : token / (uint32_t)ix.page_size;
+}
+
+// Element offset of token `token`, head 0, in page `page` (what the table says), or -1 when that page does not exist.
+JQ_HOST_DEVICE int64_t kv_offset(const KvIndex &ix, uint32_t token, int32_t page) {
+    if ((uint32_t)page >= (uint32_t)ix.num_pages) return -1;
+    const uint32_t slot = token - kv_page_of(ix, token) * (uint32_t)ix.page_size;
+    return (int64_t)page * ix.stride_page + (int64_t)slot * ix.stride_slot;
+}
+
+// Tokens of a sequence that has `len` of them by the caller's count: what fits in its row of the table.
+JQ_HOST_DEVICE int32_t kv_length(const KvIndex &ix, int32_t len) {
+    const int64_t most = (int64_t)ix.max_pages * ix.page_size;
+    return len < 0 ? 0 : len > most ? (int32_t)most : len;
+}
+
+// A turn is 2^64 steps.  `steps` per position times the position, modulo a turn, is exact; the result is in half turns, [-1, 1), and
+// off by 2^-32 from the cut and by half a bit of its own from the conversion.
+JQ_HOST_DEVICE float rope_half_turns(uint64_t steps, int32_t position) {
+    const uint64_t angle = steps * (uint64_t)(int64_t)position;
+    return (float)(int32_t)(angle >> 32) * 4.656612873077393e-10f;  // 2^-31
+}
+
+}  // namespace jq
