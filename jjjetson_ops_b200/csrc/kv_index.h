@@ -17,11 +17,21 @@ struct KvIndex {
     int64_t table_stride;
     int64_t stride_page, stride_slot, stride_head;  // in elements
     int32_t num_seqs, max_pages, num_pages, page_size;
-    int32_t page_shift;  // log2 of page_size where it is a power of two, else -1: a general division costs some 20 instructions
+    // token / page_size = token * page_magic / 2^(31 + page_shift): a division costs some 20 instructions, and the page comes first
+    uint32_t page_magic;
+    int32_t page_shift;
 };
 
+// With 2^(s - 1) < d <= 2^s and m = floor(2^(31 + s) / d) + 1, m * d is above 2^(31 + s) by at most 2^s, so that t * m / 2^(31 + s) is
+// above t / d by less than 1 / d for t < 2^31: the whole part is the quotient's.  m < 2^32 but for d = 1, where it is 2^31 + 1.
+JQ_HOST_DEVICE void kv_set_page_size(KvIndex &ix, int32_t page_size) {
+    ix.page_size = page_size;
+    ix.page_shift = 0;
+    while (((int64_t)1 << ix.page_shift) < page_size) ++ix.page_shift;
+    ix.page_magic = (uint32_t)(((uint64_t)1 << (31 + ix.page_shift)) / (uint32_t)page_size + 1);
+}
 JQ_HOST_DEVICE uint32_t kv_page_of(const KvIndex &ix, uint32_t token) {
-    return ix.page_shift >= 0 ? token >> ix.page_shift : token / (uint32_t)ix.page_size;
+    return (uint32_t)(((uint64_t)token * ix.page_magic) >> 31 >> ix.page_shift);
 }
 
 // Element offset of token `token`, head 0, in page `page` (what the table says), or -1 when that page does not exist.

@@ -11,11 +11,12 @@
 // Queries and probabilities are fp32 and are multiplied as the sum of two fp16 or three bf16 numbers (22 and 24 bits), whose products
 // with a 16-bit element are exact; so nothing is rounded to fewer than 22 bits, and the sums are fp32.
 //
-// The work is cut into units of 16 keys of one row and key head, all units of the call laid end to end, and every block takes an equal
-// stretch: long and short rows need no plan on the host, and lengths stay on the device.  The warps of a block take its units in turn, each
-// with a ring of stages of its own (asynchronous 16-byte copies) that runs on across the ends of rows.  Where a block's stretch holds all
-// of a row's key head it writes the output, else its part; the block that finds itself the last of a row's adds the parts, in
-// their order, so the result does not depend on who came last.
+// The work is cut into units of 16 keys of one row and key head, all units of the call laid end to end, and every warp takes an equal
+// stretch: long and short rows need no plan on the host, and lengths stay on the device.  A warp needs no other one until its stretch
+// is done: it has a ring of tiles of its own (asynchronous 16-byte copies), which runs on across the ends of rows, and what it has of a
+// row that begins or ends with another warp it leaves in shared memory.  Then the block puts those parts together, and where a row goes
+// on in another block leaves its part in the workspace; the block that finds itself the last of a row's adds the parts, in their order,
+// so the result does not depend on who came last.
 #include "kv_cache.cuh"
 
 #include <cmath>
@@ -24,9 +25,9 @@ namespace jq {
 
 namespace {
 
-constexpr int UNIT = 16;          // keys
-constexpr int RING_BYTES = 192 * 1024;
-constexpr int MAX_BLOCKS = 256;   // parts that the last block can weigh in its shared memory
+constexpr int UNIT = 16;          // keys; what the work is divided by
+constexpr int STEP = 2;           // units that a warp takes at a time: two tiles of 16 rows for the tensor cores
+constexpr int SMEM_BYTES = 227 * 1024;
 
 struct AttnArgs {
     const float *q;
@@ -36,7 +37,8 @@ struct AttnArgs {
     const int32_t *lens, *seqs;
     float *out;
     uint8_t *xq;
-    float scale_log2;  // scale * k_scale / ln 2
+    float scale_log2;   // |scale| * k_scale / ln 2, not zero
+    uint32_t negative;  // scale is
     float v_scale;
     int rows, q_heads, kv_heads, group, dim, window;
     int tiles;         // parts of a group that are computed apart (groups of more heads than one pass takes)
@@ -46,21 +48,27 @@ struct AttnArgs {
     float *parts;
     float2 *norms;     // [rows][q_heads]: largest logit, 1 / sum (with weights)
     float *logits;     // [rows][kv_heads][positions][group] (with weights)
-    int64_t positions;
+    int positions;     // that a row of the page table has room for
+    bool grouped;      // pages hold whole units
     int *fault;
 };
 
 // ---- element types: how 16 keys x 16 elements become operands ---------------------------------------------
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
+// d += a b, or d = a b
+#define JQ_MMA(name, types)                                                                                                              \
+    __device__ __forceinline__ void name(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {                                \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                  \
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                                             \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));                                                         \
+    }                                                                                                                                    \
+    __device__ __forceinline__ void name##_first(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {                        \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." types ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"              \
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                                             \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));                                               \
+    }
+JQ_MMA(mma_f16, "f16.f16")
+JQ_MMA(mma_bf16, "bf16.bf16")
+#undef JQ_MMA
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -69,7 +77,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
     return d;
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
@@ -90,7 +98,7 @@ struct Parts<KvF16> {
         w[0] = *reinterpret_cast<const uint32_t *>(&h);
         w[1] = *reinterpret_cast<const uint32_t *>(&l);
     }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) { mma_f16(d, a, b); }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], bool first) { first ? mma_f16_first(d, a, b) : mma_f16(d, a, b); }
 };
 template <>
 struct Parts<KvE4m3> : Parts<KvF16> {};  // e4m3 elements become fp16, exactly
@@ -107,13 +115,25 @@ struct Parts<KvBf16> {
             w[i] = *reinterpret_cast<const uint32_t *>(&h);
         }
     }
-    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) { mma_bf16(d, a, b); }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], bool first) { first ? mma_bf16_first(d, a, b) : mma_bf16(d, a, b); }
 };
 
-__device__ __forceinline__ uint32_t half2_of_e4m3(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-    return (uint32_t)h.x | (uint32_t)h.y << 16;
+// the two pairs of e4m3 in a register as two pairs of fp16
+__device__ __forceinline__ void halves_of_e4m3(uint32_t four, uint32_t &low, uint32_t &high) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(four));
 }
+// 2^x to 2^-22 of its value; 0 for -infinity and for what is below 2^-126
+__device__ __forceinline__ float power2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One warp's part of a piece, by its place in the order: where the piece lies, and where the part does.
+struct Entry {
+    int row, segment, unit, n, units;  // units [unit, unit + n) of the row's
+    int at;                            // where they lie in the block's stretch
+};
 
 // Shapes of one instance.
 template <typename T, int DP_, int NT_>
@@ -121,29 +141,40 @@ struct Shape {
     static constexpr int DP = DP_;                  // head_dim, padded
     static constexpr int NT = NT_;                  // tiles of eight heads
     static constexpr int HEADS = 8 * NT;
-    static constexpr int WARPS = DP == 256 ? 4 : 8; // a warp's accumulators and queries are its registers' larger part
+    // A warp's accumulators and queries are its registers' larger part.  8-bit tiles are half as long on their way and need conversion: twelve
+    // warps (168 registers) where they fit, eight of them 110 us against 98 for 64 sequences of up to 5000 tokens.
+    static constexpr int WARPS = NT * DP >= 256 ? 4 : sizeof(typename T::Element) == 1 && NT == 1 && DP == 128 ? 12 : 8;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROW = DP * (int)sizeof(typename T::Element);  // bytes
     static constexpr int CHUNKS = ROW / 16;
-    static constexpr int TILE = UNIT * ROW;         // keys, or values, of a unit
-    static constexpr int STAGES = RING_BYTES / (WARPS * 2 * TILE);
-    static constexpr int RED = NT == 1 ? WARPS : WARPS / 2;  // warps whose results lie in shared memory at a time
-    static constexpr int PITCH = DP + 4;            // floats; eight rows' eight elements then lie in different banks
-    static constexpr int RING = WARPS * STAGES * 2 * TILE;
-    static constexpr int RED_BYTES = RED * HEADS * PITCH * 4;
-    static constexpr int STATS = WARPS * HEADS * 8;
-    static constexpr int SMEM = RING + RED_BYTES + STATS + WARPS * STAGES * 4;
-    static constexpr int PART = HEADS * DP + 2 * HEADS;  // floats of a part: sums, then largest logits, then sums of weights
-    static_assert(STAGES >= 3, "a ring of three stages at least");
-    static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(RED_BYTES >= MAX_BLOCKS * HEADS * 4, "the parts' factors take the place of the warps' results");
+    static constexpr int KEYS = STEP * UNIT;
+    static constexpr int TILE = KEYS * ROW;         // keys, or values, of a step
+    static constexpr int RESULT = HEADS * DP * 4 + HEADS * 8;  // a warp's result: sums, then per head the largest logit and the sum of weights
+    static constexpr int FIXED = WARPS * (RESULT + 2 * (int)sizeof(Entry) + 32) + 16;
+    static constexpr int FIT = (SMEM_BYTES - FIXED) / (WARPS * TILE);
+    static constexpr int SLOTS = FIT < 6 ? FIT : 6;
+    static constexpr int RING = WARPS * SLOTS * TILE;
+    static constexpr int SMEM = RING + FIXED;
+    static constexpr int PART = HEADS * DP + 2 * HEADS;  // floats of a part: as a result
+    static constexpr bool EARLY_QUERIES = NT * DP <= 128 && WARPS <= 8;  // the others' registers are full
+    static constexpr int LEAST = WARPS * STEP;      // units of a block at least: a step for every warp
+    static_assert(SLOTS >= 3, "while one tile is read two are on their way");
+    static_assert(SLOTS * TILE >= RESULT + 2 * WARPS * HEADS * 12, "a warp's last result takes the place of its ring, the block's factors what is behind it");
+    static_assert(2 * WARPS * HEADS <= THREADS, "a thread for every factor");
 };
 
-// 16-byte chunk `c` of row `r` of a tile: spread so that eight rows' same chunk lies in different banks.
+// Where element `d` of head `h` of a result lies: eight rows' eight elements in different banks, four elements together.
+template <int DP>
+__device__ __forceinline__ int result_at(int h, int d) {
+    return h * DP + (d ^ ((h >> 1 & 3) << 3));
+}
+
+// Within a tile the 16-byte chunks of a row are spread so that eight rows' same chunk lies in different banks: chunk c of row r lies at
+// c ^ spread(r).  Addresses of other chunks and rows follow from a lane's own by constants: an exclusive or within the row (tiles begin at
+// multiples of a row), then an addition.
 template <int CHUNKS>
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-    const int x = CHUNKS >= 8 ? (r & 7) : ((r >> 1) & (CHUNKS - 1));
-    return (uint32_t)((r * CHUNKS + (c ^ x)) * 16);
+__device__ __forceinline__ constexpr int spread(int r) {
+    return CHUNKS >= 8 ? (r & 7) : ((r >> 1) & (CHUNKS - 1));
 }
 
 // What a row sees.
@@ -155,51 +186,71 @@ __device__ __forceinline__ Row row_of(const AttnArgs &a, int row) {
     Row r;
     r.seq = a.seqs != nullptr ? a.seqs[row] : row;
     if ((uint32_t)r.seq >= (uint32_t)a.ix.num_seqs) r.seq = -1;
-    r.end = r.seq < 0 ? 0 : kv_length(a.ix, a.lens[row]);
+    r.end = r.seq < 0 ? 0 : max(0, min(a.lens[row], a.positions));
     r.first = a.window > 0 && r.end > a.window ? r.end - a.window : 0;
     r.unit0 = r.first / UNIT;
     r.units = r.end > 0 ? (r.end + UNIT - 1) / UNIT - r.unit0 : 0;
     return r;
 }
 
-// Inclusive sum over the block; `partial`: one value per warp.  Every thread of the block calls it.
-template <int WARPS>
-__device__ __forceinline__ int64_t block_inclusive(int64_t v, int64_t *partial, int64_t *total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Inclusive sum over the warp.
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, v, o);
         if (lane >= o) v += u;
     }
-    __syncthreads();
-    if (lane == 31) partial[warp] = v;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += partial[w];
-        all += partial[w];
+    return v;
+}
+// Rows lie end to end, `count(row)` things each: the row in which thing `at` lies, and how many are before it there.  Every warp looks for
+// itself (no barrier); `own`: the row of the lane's number, `at` is below the sum (else the row is nonsense, and within the table).
+template <typename F>
+__device__ __forceinline__ int find_row(const AttnArgs &a, const Row &own, uint32_t at, F &&count, uint32_t *within) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int r0 = 0;; r0 += 32) {
+        const uint32_t n = r0 + lane < a.rows ? (uint32_t)count(r0 == 0 ? own : row_of(a, r0 + lane)) : 0;
+        const uint32_t end = warp_inclusive(n);
+        const uint32_t behind = __ballot_sync(0xFFFFFFFFu, at < end);
+        if (behind != 0 || r0 + 32 >= a.rows) {
+            const int i = behind != 0 ? __ffs(behind) - 1 : 0;
+            *within = at - __shfl_sync(0xFFFFFFFFu, end - n, i);
+            return r0 + i;
+        }
+        at -= __shfl_sync(0xFFFFFFFFu, end, 31);
     }
-    *total = all;
-    return v + before;
+}
+__device__ __forceinline__ Row row_at(const AttnArgs &a, const Row &own, int row) {
+    if (row >= 32) return row_of(a, row);
+    Row r;
+    r.seq = __shfl_sync(0xFFFFFFFFu, own.seq, row);
+    r.first = __shfl_sync(0xFFFFFFFFu, own.first, row);
+    r.end = __shfl_sync(0xFFFFFFFFu, own.end, row);
+    r.units = __shfl_sync(0xFFFFFFFFu, own.units, row);
+    r.unit0 = __shfl_sync(0xFFFFFFFFu, own.unit0, row);
+    return r;
 }
 
 // Four consecutive elements of the output: element `e` of the heads of one key head's tile (their elements lie end to end), as
-// fp32 and as Q8_1.  Every lane of the warp calls it, with consecutive e; `there`: it has elements.
-__device__ __forceinline__ void write_output(const AttnArgs &a, int row, int head0, int e, float4 v, bool there) {
-    const int64_t n = (int64_t)head0 * a.dim + e;  // within the row
-    if (a.out != nullptr && there) *reinterpret_cast<float4 *>(a.out + (int64_t)row * a.q_heads * a.dim + n) = v;
-    if (a.xq != nullptr) {
-        if (!there) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t ds;
-        const uint32_t q = quantize_group_q8_1(v, a.s_mode, &ds);
-        if (there) {
-            uint8_t *block = a.xq + q8_block_index(n / SUPER, row, a.n_super, a.rows, a.order) * Q8_BYTES;
-            const int i = (int)(n % SUPER);
-            *reinterpret_cast<uint32_t *>(block + Q8_QS_OFFSET + i) = q;
-            if (i % QK == 0) *reinterpret_cast<uint32_t *>(block + i / QK * 4) = ds;
-        }
+// fp32 and as Q8_1.  Every lane of the warp calls it, with consecutive e; `there`: it has elements.  (Not inlined: the kernel's instructions
+// have to stay in the SM's cache.  147 KB of them, with everything inlined, made a call of one short sequence take 12.6 us, most of it
+// waiting for instructions.)
+__device__ __noinline__ void write_q8(uint8_t *xq, int n, int row, int n_super, int rows, int order, int s_mode, float4 v, bool there) {
+    if (!there) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint32_t ds;
+    const uint32_t q = quantize_group_q8_1(v, s_mode, &ds);
+    if (there) {
+        uint8_t *block = xq + q8_block_index(n / SUPER, row, n_super, rows, order) * Q8_BYTES;
+        const int i = n % SUPER;
+        *reinterpret_cast<uint32_t *>(block + Q8_QS_OFFSET + i) = q;
+        if (i % QK == 0) *reinterpret_cast<uint32_t *>(block + i / QK * 4) = ds;
     }
+}
+__device__ __forceinline__ void write_output(const AttnArgs &a, int row, int head0, int e, float4 v, bool there) {
+    const int n = head0 * a.dim + e;  // within the row
+    if (a.out != nullptr && there) *reinterpret_cast<float4 *>(a.out + (int64_t)row * a.q_heads * a.dim + n) = v;
+    if (a.xq != nullptr) write_q8(a.xq, n, row, a.n_super, a.rows, a.order, a.s_mode, v, there);
 }
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }  // a row whose pages are all bad gives zeros
@@ -208,16 +259,14 @@ template <typename T, int DP, int NT, bool WEIGHTS>
 __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_kernel(const AttnArgs a) {
     using S = Shape<T, DP, NT>;
     using P = Parts<T>;
-    constexpr bool E4M3 = sizeof(typename T::Element) == 1;
+    using E = typename T::Element;
+    constexpr bool E4M3 = sizeof(E) == 1;
     constexpr int W = S::WARPS;
-    extern __shared__ __align__(128) unsigned char smem[];
-    float *red = reinterpret_cast<float *>(smem + S::RING);
-    float2 *stats = reinterpret_cast<float2 *>(smem + S::RING + S::RED_BYTES);  // [warp][head]: largest logit, sum
-    uint32_t *masks = reinterpret_cast<uint32_t *>(smem + S::RING + S::RED_BYTES + S::STATS);
-    __shared__ int64_t partial[W];
-    __shared__ int start_row;
-    __shared__ int64_t start_unit;
-    __shared__ int is_last;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char *results = smem + S::RING;  // one per warp: of a row that began with another warp
+    Entry *entries = reinterpret_cast<Entry *>(results + W * S::RESULT);  // two per warp: that, and its last piece
+    uint32_t *masks = reinterpret_cast<uint32_t *>(entries + 2 * W);
+    int *is_last = reinterpret_cast<int *>(masks + 8 * W);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -225,160 +274,286 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     const int segments_row = a.kv_heads * a.tiles;  // a row's key heads, or tiles of their query heads: each has the row's units
 
     // ---- the block's stretch ----
-    int64_t total = 0;
-    for (int r0 = 0; r0 < a.rows; r0 += S::THREADS) {
-        const int r = r0 + threadIdx.x;
-        int64_t all;
-        (void)block_inclusive<W>(r < a.rows ? (int64_t)row_of(a, r).units * segments_row : 0, partial, &all);
-        total += all;
+    Row own = {-1, 0, 0, 0, 0};  // the row of this lane's number
+    if (lane < a.rows) own = row_of(a, lane);
+    uint32_t total = own.units * segments_row, segments = own.units > 0 ? segments_row : 0;
+#pragma unroll 1
+    for (int r = lane + 32; r < a.rows; r += 32) {
+        const uint32_t n = row_of(a, r).units;
+        total += n * segments_row;
+        segments += n > 0 ? segments_row : 0;
     }
-    int64_t per_block = (total + gridDim.x - 1) / gridDim.x;
-    if (per_block < W) per_block = W;  // a unit for every warp: fewer parts to add
-    const int64_t u0 = blockIdx.x * per_block, u1 = min(total, u0 + per_block);
-    // rows that see nothing get their zeros here
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const Row x = row_of(a, r);
-        if (x.seq < 0 || x.units > 0) continue;
-        const int n4 = a.q_heads * a.dim / 4;
-        for (int e = threadIdx.x; e < (n4 + 31) / 32 * 32; e += S::THREADS)
-            write_output(a, r, 0, 4 * e, make_float4(0.f, 0.f, 0.f, 0.f), e < n4);
-    }
-    if (u0 >= u1) return;
-    {
-        int64_t before = 0;
-        for (int r0 = 0; r0 < a.rows; r0 += S::THREADS) {
-            const int r = r0 + threadIdx.x;
-            const int64_t n = r < a.rows ? (int64_t)row_of(a, r).units * segments_row : 0;
-            int64_t all;
-            const int64_t end = before + block_inclusive<W>(n, partial, &all);
-            if (end - n <= u0 && u0 < end) start_row = r, start_unit = u0 - (end - n);
-            before += all;
-            if (before > u0) break;
-        }
-        __syncthreads();
-    }
-    const int count = (int)(u1 - u0);  // units of this block; the host has bounded it
-
-    // ---- the ring: every lane knows where one key of the unit that is copied next lies ----
-    const uint32_t ring = smem_u32(smem) + warp * S::STAGES * 2 * S::TILE;
-    uint32_t *mask_ring = masks + warp * S::STAGES;
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    segments = __reduce_add_sync(0xFFFFFFFFu, segments);
+    // Few segments: each gets blocks of its own, so that a block has one segment to put together; at most an eighth of the blocks stay
+    // idle.  Many: equal stretches.
+    const bool apart = segments * 8 <= gridDim.x;
+    uint32_t per_block = apart ? (total + gridDim.x - segments - 1) / (gridDim.x - segments) : (total + gridDim.x - 1) / gridDim.x;
+    if (per_block < S::LEAST) per_block = S::LEAST;
+    const uint32_t u0 = blockIdx.x * per_block;  // (not apart)
+    int count = 0;                               // units of this block
+    int first_block = 0, parts_apart = 1;
     struct {
         Row row;
-        int r, segment, unit;  // unit within the row's
-        int left;
-        int64_t offset;        // bytes, of this lane's key (lanes 0 to 15)
-        bool there;
-    } next;
-    next.r = start_row;
-    next.row = row_of(a, next.r);
-    next.segment = (int)(start_unit / next.row.units);
-    next.unit = (int)(start_unit - (int64_t)next.segment * next.row.units);
-    next.left = count > warp ? (count - warp + W - 1) / W : 0;
-    const auto advance = [&](int n) {
-        next.unit += n;
-        while (next.unit >= next.row.units) {
-            next.unit -= next.row.units;
-            if (++next.segment == segments_row) {
-                next.segment = 0;
-                do {
-                    next.row = row_of(a, ++next.r);
-                } while (next.row.units == 0);
+        int r, segment, unit;
+    } piece = {};  // the warp's first
+    int a0 = 0, a1 = 0;  // the warp's stretch within the block's
+    if (apart) {
+        uint32_t within;
+        piece.r = find_row(a, own, blockIdx.x, [&](const Row &r) { return segments_row * ((r.units + per_block - 1) / per_block); }, &within);
+        if (piece.r < a.rows) {
+            piece.row = row_at(a, own, piece.r);
+            parts_apart = (piece.row.units + per_block - 1) / per_block;
+            if (within < (uint32_t)(segments_row * parts_apart)) {
+                piece.segment = within / parts_apart;
+                const int part = within - piece.segment * parts_apart;
+                const int each = (piece.row.units + parts_apart - 1) / parts_apart;
+                first_block = blockIdx.x - part;
+                piece.unit = part * each;
+                count = max(0, min(piece.row.units - piece.unit, each));
+                parts_apart = (piece.row.units + each - 1) / each;  // (rounded up, `each` may leave nothing to the last blocks)
             }
         }
-    };
-    const auto locate = [&]() {  // asks the page table for the unit after the one that is being copied
-        const int key = (next.row.unit0 + next.unit) * UNIT + lane;
-        next.there = false;
-        next.offset = 0;
-        if (lane < UNIT && key >= next.row.first && key < next.row.end) {
-            const int64_t to = kv_offset(a.ix, (uint32_t)key, a.ix.table[(int64_t)next.row.seq * a.ix.table_stride + kv_page_of(a.ix, (uint32_t)key)]);
-            next.there = to >= 0;
-            if (to < 0) report_bad_page(a.fault);
-            else next.offset = (to + (int64_t)(next.segment / a.tiles) * a.ix.stride_head) * (int)sizeof(typename T::Element);
+        a0 = warp * count / W, a1 = (warp + 1) * count / W;
+        piece.unit += a0;
+    } else if (u0 < total) {
+        count = min(per_block, total - u0);
+        a0 = warp * count / W, a1 = (warp + 1) * count / W;
+        if (a0 < a1) {
+            uint32_t within;
+            piece.r = find_row(a, own, u0 + a0, [&](const Row &r) { return segments_row * r.units; }, &within);
+            piece.row = row_at(a, own, piece.r);
+            piece.segment = within / piece.row.units;
+            piece.unit = within - piece.segment * piece.row.units;
         }
-    };
-    const auto copy = [&](int stage) {
-        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, next.there);
-        if (lane == 0) mask_ring[stage] = mask;
-        const uint32_t to = ring + stage * 2 * S::TILE;
-        const int c = lane % S::CHUNKS;
-        const bool inside = c * 16 < a.dim * (int)sizeof(typename T::Element);
-        constexpr int AT_ONCE = 32 / S::CHUNKS;
-#pragma unroll
-        for (int i = 0; i < UNIT / AT_ONCE; ++i) {
-            const int r = lane / S::CHUNKS + i * AT_ONCE;
-            const int64_t offset = __shfl_sync(0xFFFFFFFFu, next.offset, r);
-            const bool there = inside && (mask >> r & 1u);
-            const int64_t at = there ? offset + c * 16 : 0;
-            copy16(to + chunk_at<S::CHUNKS>(r, c), a.k + at, there);
-            copy16(to + S::TILE + chunk_at<S::CHUNKS>(r, c), a.v + at, there);
-        }
-    };
-    const auto copy_next = [&](int stage) {
-        if (next.left > 0) {
-            copy(stage);
-            if (--next.left > 0) {
-                advance(W);
-                locate();
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    if (next.left > 0) {
-        if (warp > 0) advance(warp);
-        locate();
     }
-#pragma unroll 1
-    for (int s = 0; s < S::STAGES - 1; ++s) copy_next(s);
-    int stage = 0;
 
-    // ---- the block's pieces of rows ----
-    int row = start_row, done = 0;
-    Row seen = row_of(a, row);
-    int segment = (int)(start_unit / seen.units);
-    int unit = (int)(start_unit - (int64_t)segment * seen.units);
+    // ---- the warp's pieces: first those that begin and end with it, then the one that began before, then the last ----
+    // (so that what it has of the first piece stays where the others' results were turned around)
+    Entry *mine = entries + 2 * warp;  // [0]: the first piece where others follow, [1]: the last; n = 0: none
+    int middle = 0;                    // units of the pieces between the two
+    {
+        const int n = a1 - a0;
+        Entry first = {piece.r, piece.segment, piece.unit, n > 0 ? min(n, piece.row.units - piece.unit) : 0, piece.row.units, a0}, last = first;
+        if (first.n < n) {
+            uint32_t within;
+            last.row = find_row(a, own, u0 + a1 - 1, [&](const Row &r) { return segments_row * r.units; }, &within);
+            last.units = row_at(a, own, last.row).units;
+            last.segment = within / last.units;
+            last.unit = 0;
+            last.n = within - last.segment * last.units + 1;
+            last.at = a1 - last.n;
+            middle = n - first.n - last.n;
+        } else {
+            first.n = 0;
+        }
+        if (lane == 0) mine[0] = first, mine[1] = last;
+        __syncwarp();
+    }
+    const bool any = a0 < a1;
+    // A walk over the pieces; `row` and the others of the piece are what the walker needs of it.
+    enum { MIDDLE, FIRST, LAST, DONE };
+    struct Walk {
+        Row row;
+        int r, segment, unit, n;  // units left of the piece, from `unit` on
+        int phase, middle;
+    };
+    const auto next_piece = [&](Walk &w) {
+        if (w.phase == MIDDLE && w.middle > 0) {  // the next segment, all of it
+            if (++w.segment == segments_row) {
+                w.segment = 0;
 #pragma unroll 1
-    while (done < count) {
-        const int piece = min(count - done, seen.units - unit);
-        const int kv_head = segment / a.tiles, tile = segment - kv_head * a.tiles;
+                do {
+                    w.row = row_of(a, ++w.r);
+                } while (w.row.units == 0);
+            }
+            w.unit = 0;
+            w.n = w.row.units;
+            w.middle -= w.n;
+        } else if (++w.phase != DONE) {
+            const Entry &e = mine[w.phase == FIRST ? 0 : 1];
+            w.r = e.row, w.segment = e.segment, w.unit = e.unit, w.n = e.n;
+            w.row = row_of(a, w.r);
+        }
+    };
+    Walk at, next;  // what is computed, and what is copied
+    at.row = piece.row, at.r = piece.r, at.segment = piece.segment, at.middle = middle;
+    at.phase = !any ? LAST : mine[0].n > 0 ? MIDDLE : FIRST;  // (the phase before that of the first piece to take)
+    next_piece(at);
+    next = at;
+
+    // queries of one piece: the elements that go with the keys' operands, 2i, 2i + 1, 2i + 8, 2i + 9 of 16, or with e4m3 the four from
+    // 4i on.  They are asked for early where there are registers: before the cache is looked up, and before the piece ahead is put away.
+    float raw[NT][DP / 16][4];
+    const auto ask_queries = [&]() {
+        const int kv_head = a.tiles == 1 ? at.segment : at.segment / a.tiles, tile = at.segment - kv_head * a.tiles;
         const int head0 = kv_head * a.group + tile * S::HEADS, heads = min(S::HEADS, a.group - tile * S::HEADS);
-
-        // queries: two or three operands per 16 elements, scaled by a power of two so that fp16 holds them
-        uint32_t q[NT][DP / 16][P::N][2];
-        float unscale[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int h = 8 * t + (lane >> 2);
-            const float *from = a.q + (int64_t)row * a.q_row + (int64_t)(head0 + h) * a.q_head;
-            float x[DP / 16][4];
-            float largest = 0.f;
+            const int h = 8 * t + (lane >> 2), i = lane & 3;
+            const float *from = a.q + (int64_t)at.r * a.q_row + (int64_t)(head0 + h) * a.q_head;
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) {
                 const bool there = h < heads && 16 * s < a.dim;
-                // the elements that go with the keys' operands: 2i, 2i + 1, 2i + 8, 2i + 9 of 16, or with e4m3 the four from 4i on
-                const int i = lane & 3;
                 if (E4M3) {
                     const float4 v = there ? *reinterpret_cast<const float4 *>(from + 16 * s + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[s][0] = v.x, x[s][1] = v.y, x[s][2] = v.z, x[s][3] = v.w;
+                    raw[t][s][0] = v.x, raw[t][s][1] = v.y, raw[t][s][2] = v.z, raw[t][s][3] = v.w;
                 } else {
                     const float2 v = there ? *reinterpret_cast<const float2 *>(from + 16 * s + 2 * i) : make_float2(0.f, 0.f);
                     const float2 u = there ? *reinterpret_cast<const float2 *>(from + 16 * s + 2 * i + 8) : make_float2(0.f, 0.f);
-                    x[s][0] = v.x, x[s][1] = v.y, x[s][2] = u.x, x[s][3] = u.y;
+                    raw[t][s][0] = v.x, raw[t][s][1] = v.y, raw[t][s][2] = u.x, raw[t][s][3] = u.y;
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fabsf(x[s][j]));
             }
+        }
+    };
+    if (S::EARLY_QUERIES && any) ask_queries();
+
+    // ---- the ring: tiles of keys and of values in turn ----
+    // A step's keys lie in pages.  Where a page holds whole units, every lane has the two units' offsets, else each lane has its own
+    // key's, and they are passed around.
+    unsigned char *const my_ring = smem + warp * S::SLOTS * S::TILE;
+    const uint32_t ring = smem_u32(my_ring);
+    uint32_t *mask_ring = masks + warp * S::SLOTS;
+    const bool grouped = a.grouped;
+    // What the page table was asked for the step that is copied next; the answer is looked at half a step later.
+    struct {
+        int key0;
+        uint32_t mask;     // which of the 32 keys are there
+        int page[2];
+        int64_t head;
+        bool live;         // a step, even if none of its keys is
+    } asked;
+    const auto ask = [&]() {
+        asked.live = next.phase != DONE;
+        if (!asked.live) return;
+        const int key0 = (next.row.unit0 + next.unit) * UNIT;
+        const int end = min(next.row.end, key0 + min(next.n, STEP) * UNIT);
+        const int32_t *table = a.ix.table + (int64_t)next.row.seq * a.ix.table_stride;
+        const uint32_t from = next.row.first > key0 ? 0xFFFFFFFFu << (next.row.first - key0) : 0xFFFFFFFFu;
+        const uint32_t until = end - key0 >= 32 ? 0xFFFFFFFFu : ~(0xFFFFFFFFu << (end - key0));
+        asked.key0 = key0;
+        asked.mask = from & until;
+        asked.head = (int64_t)(a.tiles == 1 ? next.segment : next.segment / a.tiles) * a.ix.stride_head;
+        asked.page[0] = asked.page[1] = 0;
+        if (grouped) {
+            asked.page[0] = table[kv_page_of(a.ix, (uint32_t)key0)];
+            if (key0 + UNIT < end) asked.page[1] = table[kv_page_of(a.ix, (uint32_t)(key0 + UNIT))];
+        } else if (asked.mask >> lane & 1u) {
+            asked.page[0] = table[kv_page_of(a.ix, (uint32_t)(key0 + lane))];
+        }
+        next.unit += STEP;
+        next.n -= STEP;
+        if (next.n <= 0) next_piece(next);
+    };
+    const int my_chunk = lane % S::CHUNKS;
+    const bool inside = my_chunk * 16 < a.dim * (int)sizeof(E);
+    constexpr int AT_ONCE = 32 / S::CHUNKS;  // rows that the warp copies with one instruction
+    const uint32_t my_place = lane / S::CHUNKS * S::ROW + (my_chunk ^ spread<S::CHUNKS>(lane / S::CHUNKS)) * 16;
+    // of the operands that this lane reads: keys (rows of the product are keys) and values (rows are elements)
+    const uint32_t k_place = (lane & 15) * S::ROW + ((lane >> 4) ^ spread<S::CHUNKS>(lane & 15)) * 16;
+    const uint32_t v_place = ((lane & 7) + (lane >> 4) * 8) * S::ROW + ((lane >> 3 & 1) ^ spread<S::CHUNKS>(lane & 7)) * 16;
+    const int64_t row_stride = a.ix.stride_slot * (int)sizeof(E);
+    const int64_t my_start = inside ? (lane / S::CHUNKS) * row_stride + my_chunk * 16 : 0;
+    struct {
+        int64_t offset[2];  // bytes, of this lane's first rows of the two units (not grouped: of its key)
+        uint32_t mask;
+        bool live;
+    } here = {};
+    // Tile 2n is the keys, 2n + 1 the values of the warp's n-th step; tile t lies in slot t % SLOTS.
+    int slot_next = S::SLOTS - 1, mask_next = 0;
+    const auto copy_next = [&](bool values) {
+        if (!values) {
+            here.live = asked.live;
+            here.mask = asked.mask;
+            const uint32_t units = grouped ? 0x0000FFFFu : 1u << lane;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const uint32_t mine_of = g == 0 ? units : ~units;
+                const int64_t to = kv_offset(a.ix, (uint32_t)(asked.key0 + (grouped ? UNIT * g : lane)), asked.page[g]);
+                here.offset[g] = (to + asked.head) * (int)sizeof(E) + (grouped ? my_start : my_chunk * 16);
+                if (to < 0) {
+                    here.offset[g] = 0;
+                    if (asked.live && (asked.mask & mine_of) != 0 && (grouped || g == 0)) report_bad_page(a.fault);
+                    if (grouped) here.mask &= ~mine_of;
+                }
+                if (!grouped && g == 0) here.mask = __ballot_sync(0xFFFFFFFFu, to >= 0) & asked.mask;
+            }
+            if (lane == 0) mask_ring[mask_next] = here.mask;
+            if (++mask_next == S::SLOTS) mask_next = 0;
+        }
+        const char *pool = values ? a.v : a.k;
+        const uint32_t to = ring + slot_next * S::TILE;
+        if (here.live) {
+            const uint32_t own = to + my_place;
+            if (grouped && here.mask == 0xFFFFFFFFu) {
+                const char *from[2] = {pool + here.offset[0], pool + here.offset[1]};
+#pragma unroll
+                for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
+                    copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, from[i * AT_ONCE / UNIT], inside);
+                    from[i * AT_ONCE / UNIT] += AT_ONCE * row_stride;
+                }
+            } else {
+                // (what is not there is not read: its offset is a place in the pool all the same)
+#pragma unroll 2
+                for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
+                    const int r = lane / S::CHUNKS + i * AT_ONCE;
+                    const int64_t other = __shfl_sync(0xFFFFFFFFu, here.offset[0], r);  // (its chunk is that lane's)
+                    const int64_t offset = grouped ? (i * AT_ONCE < UNIT ? here.offset[0] : here.offset[1]) + (i * AT_ONCE % UNIT) * row_stride
+                                                   : other - (r % S::CHUNKS) * 16 + my_chunk * 16;
+                    const bool there = inside && (here.mask >> r & 1u);
+                    copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, pool + (there ? offset : 0), there);
+                }
+            }
+        }
+        if (values) ask();
+        if (++slot_next == S::SLOTS) slot_next = 0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    // A new tile goes into the slot of the one that was read before, then the oldest is waited for and read.
+    constexpr bool SAME = (S::SLOTS & 1) != 0;  // what is copied while keys are read: keys, else values
+    asked.live = false;
+#pragma unroll 1
+    for (int t = -1; t < S::SLOTS - 1; ++t) copy_next(t & 1);  // (the values of a step before the first, which is none: the page table is asked there)
+    int slot = 0, mask_slot = 0;
+    const auto next_tile = [&](bool values) {
+        __syncwarp();
+        copy_next(values == SAME);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::SLOTS - 1) : "memory");
+        __syncwarp();
+        const uint32_t tile = ring + slot * S::TILE;
+        if (++slot == S::SLOTS) slot = 0;
+        return tile;
+    };
+
+#pragma unroll 1
+    while (at.phase != DONE) {
+        const int kv_head = a.tiles == 1 ? at.segment : at.segment / a.tiles, tile_of = at.segment - kv_head * a.tiles;
+        const int head0 = kv_head * a.group + tile_of * S::HEADS, heads = min(S::HEADS, a.group - tile_of * S::HEADS);
+        uint32_t q[NT][DP / 16][P::N][2];
+        float unscale[NT][2];
+        float o[NT][DP / 16][4];
+        float m[NT][2], l[NT][2];
+        // queries: two or three operands per 16 elements, scaled by a power of two so that fp16 holds them
+        if (!S::EARLY_QUERIES) ask_queries();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float largest = 0.f;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fabsf(raw[t][s][j]));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2));
             // 2^-e with 2^e <= largest, within 2^-100 .. 2^100
             int e = (int)(__float_as_uint(largest) >> 23) - 127;
             e = P::N == 3 || largest == 0.f ? 0 : max(-100, min(100, e));
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23 | a.negative << 31), up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) {
                 uint32_t w0[P::N], w1[P::N];
-                P::split(x[s][0] * down, x[s][1] * down, w0);
-                P::split(x[s][2] * down, x[s][3] * down, w1);
+                P::split(raw[t][s][0] * down, raw[t][s][1] * down, w0);
+                P::split(raw[t][s][2] * down, raw[t][s][3] * down, w1);
 #pragma unroll
                 for (int j = 0; j < P::N; ++j) q[t][s][j][0] = w0[j], q[t][s][j][1] = w1[j];
             }
@@ -386,9 +561,6 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
             unscale[t][0] = __shfl_sync(0xFFFFFFFFu, up, 8 * (lane & 3));
             unscale[t][1] = __shfl_sync(0xFFFFFFFFu, up, 8 * (lane & 3) + 4);
         }
-
-        float o[NT][DP / 16][4];
-        float m[NT][2], l[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             m[t][0] = m[t][1] = -INFINITY;
@@ -399,129 +571,165 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 for (int j = 0; j < 4; ++j) o[t][s][j] = 0.f;
         }
 
-        int mine = (warp - done % W + W) % W;  // this warp's first unit of the piece
 #pragma unroll 1
-        for (; mine < piece; mine += W) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
-            __syncwarp();
-            const uint32_t kt = ring + stage * 2 * S::TILE, vt = kt + S::TILE;
-            const uint32_t mask = mask_ring[stage];
-            // the stage that was read in the step before this one takes the next unit
-            copy_next(stage == 0 ? S::STAGES - 1 : stage - 1);
-
-            // logits of 16 keys x 8 NT heads; four sums, so that no product waits for all the others
-            float s4[NT][4][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s4[t][i][j] = 0.f;
+        for (int u = 0; u < at.n; u += STEP) {
+            uint32_t tile = next_tile(false);
+            const uint32_t mask = mask_ring[mask_slot];
+            if (++mask_slot == S::SLOTS) mask_slot = 0;
+            uint32_t p[NT][2][P::N][2];
+            float shrink[NT][2];
+            // logits of 2 x 16 keys x 8 NT heads: of the queries' largest parts, and of the others
+            float s4[NT][2][2][4];
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) {
-                uint32_t k[4];
                 if constexpr (E4M3) {
                     if (s & 1) continue;
-                    uint32_t r[4];
-                    ldmatrix4(r, kt + chunk_at<S::CHUNKS>(lane & 15, s + (lane >> 4)));
+                    uint32_t r[2][4];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t k8[4] = {half2_of_e4m3(r[2 * u] & 0xFFFFu), half2_of_e4m3(r[2 * u + 1] & 0xFFFFu),
-                                                half2_of_e4m3(r[2 * u] >> 16), half2_of_e4m3(r[2 * u + 1] >> 16)};
+                    for (int g = 0; g < 2; ++g) ldmatrix4(r[g], ((tile + k_place) ^ (s * 16)) + UNIT * g * S::ROW);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
+                    for (int v = 0; v < 2; ++v) {
+                        uint32_t k8[2][4];
 #pragma unroll
-                            for (int j = 0; j < P::N; ++j) P::mma(s4[t][(2 * u + j) & 3], k8, q[t][s + u][j]);
+                        for (int g = 0; g < 2; ++g) {
+                            halves_of_e4m3(r[g][2 * v], k8[g][0], k8[g][2]);
+                            halves_of_e4m3(r[g][2 * v + 1], k8[g][1], k8[g][3]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < P::N; ++j)
+#pragma unroll
+                            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                for (int t = 0; t < NT; ++t) P::mma(s4[t][g][j > 0 ? 1 : 0], k8[g], q[t][s + v][j], s + v == 0 && j < 2);
                     }
                 } else {
-                    ldmatrix4(k, kt + chunk_at<S::CHUNKS>(lane & 15, 2 * s + (lane >> 4)));
+                    uint32_t k[2][4];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                    for (int g = 0; g < 2; ++g) ldmatrix4(k[g], ((tile + k_place) ^ (s * 32)) + UNIT * g * S::ROW);
 #pragma unroll
-                        for (int j = 0; j < P::N; ++j) P::mma(s4[t][(P::N * s + j) & 3], k, q[t][s][j]);
+                    for (int j = 0; j < P::N; ++j)
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) P::mma(s4[t][g][j > 0 ? 1 : 0], k[g], q[t][s][j], s == 0 && j < 2);
                 }
             }
-
-            const bool v0 = mask >> (lane >> 2) & 1u, v1 = mask >> ((lane >> 2) + 8) & 1u;
-            uint32_t p[NT][P::N][2];
-            float shrink[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float x[4];
+                // x: products of the scaled queries; logits in base 2 are x times unscale (which is positive)
+                float x[2][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float sum = (s4[t][0][j] + s4[t][1][j]) + (s4[t][2][j] + s4[t][3][j]);
-                    x[j] = (j < 2 ? v0 : v1) ? sum * unscale[t][j & 1] : -INFINITY;
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[g][j] = s4[t][g][0][j] + s4[t][g][1][j];
+                if (mask != 0xFFFFFFFFu) {
+                    const uint32_t seen = mask >> (lane >> 2);
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[g][j] = seen >> (16 * g + 8 * (j >> 1)) & 1u ? x[g][j] : -INFINITY;
                 }
                 if (WEIGHTS) {
-                    const int64_t key = (int64_t)(seen.unit0 + unit + mine) * UNIT + (lane >> 2);
-                    const int64_t base = ((int64_t)row * a.kv_heads + kv_head) * a.positions;
-                    const int h = tile * S::HEADS + 8 * t + 2 * (lane & 3);
+                    const int kv_head = a.tiles == 1 ? at.segment : at.segment / a.tiles;
+                    const int h = (at.segment - kv_head * a.tiles) * S::HEADS + 8 * t + 2 * (lane & 3);
+                    const int key = (at.row.unit0 + at.unit + u) * UNIT + (lane >> 2);
+                    const int end = min(at.row.end, (at.row.unit0 + at.unit + at.n) * UNIT);
+                    float *to = a.logits + (((int64_t)at.r * a.kv_heads + kv_head) * a.positions + key) * a.group + h;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const bool in = key + 8 * (j >> 1) >= seen.first && key + 8 * (j >> 1) < seen.end;
-                        if (in && h + (j & 1) < a.group) a.logits[(base + key + 8 * (j >> 1)) * a.group + h + (j & 1)] = x[j];
-                    }
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int more = 16 * g + 8 * (j >> 1);
+                            if (key + more >= at.row.first && key + more < end && h + (j & 1) < a.group) to[more * a.group + (j & 1)] = x[g][j] * unscale[t][j & 1];
+                        }
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float top = fmaxf(x[j], x[j + 2]);
+                    float top = fmaxf(fmaxf(x[0][j], x[0][j + 2]), fmaxf(x[1][j], x[1][j + 2]));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                    top = fmaxf(top, m[t][j]);
-                    const float from = top == -INFINITY ? 0.f : top;  // keys of bad pages only, so far
-                    shrink[t][j] = exp2f(m[t][j] - from);
+                    const float c = unscale[t][j];
+                    top = fmaxf(top * c, m[t][j]);
+                    const float from = top == -INFINITY ? 0.f : -top;  // (keys of bad pages only, so far)
+                    shrink[t][j] = power2(m[t][j] + from);
                     m[t][j] = top;
-                    x[j] = exp2f(x[j] - from) * P::UP;
-                    x[j + 2] = exp2f(x[j + 2] - from) * P::UP;
-                    l[t][j] = l[t][j] * shrink[t][j] + (x[j] + x[j + 2]);
-                }
-                uint32_t w0[P::N], w1[P::N];
-                P::split(x[0], x[1], w0);
-                P::split(x[2], x[3], w1);
+                    float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < P::N; ++j) p[t][j][0] = transposed(w0[j]), p[t][j][1] = transposed(w1[j]);
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int i = j; i < 4; i += 2) {
+                            x[g][i] = power2(fmaf(x[g][i], c, from)) * P::UP;
+                            sum += x[g][i];
+                        }
+                    l[t][j] = l[t][j] * shrink[t][j] + sum;
+                }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t w0[P::N], w1[P::N];
+                    P::split(x[g][0], x[g][1], w0);
+                    P::split(x[g][2], x[g][3], w1);
+#pragma unroll
+                    for (int j = 0; j < P::N; ++j) p[t][g][j][0] = transposed(w0[j]), p[t][g][j][1] = transposed(w1[j]);
+                }
             }
 
-            // the tensor cores cut a sum's last bits off instead of rounding: they add up one unit, the sum over units is rounded
+            tile = next_tile(true);
+            // The tensor cores cut a sum's last bits off instead of rounding: they add up one step, the sum over steps is rounded.  The small
+            // parts go first.  Four tiles of 16 elements at a time, so that four sums are in the making.
+            constexpr int BATCH = NT == 1 && W <= 8 ? 4 : 2;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-                uint32_t v[4];
+            for (int s0 = 0; s0 < DP / 16; s0 += BATCH) {
+                float d[BATCH][NT][4];
+                uint32_t v[BATCH][2][4];
                 if constexpr (E4M3) {
-                    if (s & 1) continue;
-                    uint32_t r[4];
-                    ldmatrix4_trans(r, vt + chunk_at<S::CHUNKS>((lane & 7) + ((lane >> 4) << 3), s + ((lane >> 3) & 1)));
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        // rows of the product: elements 2i, then 2i + 1, of the 16
-                        const uint32_t a0 = __byte_perm(r[u], 0, 0x3120), a1 = __byte_perm(r[u + 2], 0, 0x3120);
-                        const uint32_t v8[4] = {half2_of_e4m3(a0 & 0xFFFFu), half2_of_e4m3(a0 >> 16), half2_of_e4m3(a1 & 0xFFFFu), half2_of_e4m3(a1 >> 16)};
+                    for (int s = 0; s < BATCH; s += 2)
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t r[4];
+                            ldmatrix4_trans(r, ((tile + v_place) ^ ((s0 + s) * 16)) + UNIT * g * S::ROW);
 #pragma unroll
-                            for (int j = P::N - 1; j >= 0; --j) P::mma(d, v8, p[t][j]);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) o[t][s + u][j] = o[t][s + u][j] * shrink[t][j & 1] + d[j];
+                            for (int k = 0; k < 2; ++k) {
+                                // rows of the product: elements 2i, then 2i + 1, of the 16
+                                halves_of_e4m3(__byte_perm(r[k], 0, 0x3120), v[s + k][g][0], v[s + k][g][1]);
+                                halves_of_e4m3(__byte_perm(r[k + 2], 0, 0x3120), v[s + k][g][2], v[s + k][g][3]);
+                            }
                         }
-                    }
                 } else {
-                    ldmatrix4_trans(v, vt + chunk_at<S::CHUNKS>((lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1)));
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int s = 0; s < BATCH; ++s)
 #pragma unroll
-                        for (int j = P::N - 1; j >= 0; --j) P::mma(d, v, p[t][j]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) o[t][s][j] = o[t][s][j] * shrink[t][j & 1] + d[j];
-                    }
+                        for (int g = 0; g < 2; ++g)
+                            ldmatrix4_trans(v[s][g], ((tile + v_place) ^ ((s0 + s) * 32)) + UNIT * g * S::ROW);
                 }
+#pragma unroll
+                for (int j = P::N - 1; j >= 0; --j)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int s = 0; s < BATCH; ++s)
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) P::mma(d[s][t], v[s][g], p[t][g][j], j == P::N - 1 && g == 0);
+#pragma unroll
+                for (int s = 0; s < BATCH; ++s)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[t][s0 + s][j] = o[t][s0 + s][j] * shrink[t][j & 1] + d[s][t][j];
             }
-            if (++stage == S::STAGES) stage = 0;
         }
 
-        // ---- the warps' results to one ----
+        // the next piece; its queries are asked for while this one is put away
+        const int row = at.r, phase = at.phase;
+        const bool whole = at.unit == 0 && at.n == at.row.units;
+        next_piece(at);
+        if (S::EARLY_QUERIES && at.phase != DONE) ask_queries();
+
+        // into shared memory, by heads: where the ring was, if this was the last piece
+        float *result = reinterpret_cast<float *>(phase == LAST ? my_ring : results + warp * S::RESULT);
+        float2 *stats = reinterpret_cast<float2 *>(result + S::HEADS * DP);
+        __syncwarp();
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -529,171 +737,218 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 l[t][j] += __shfl_xor_sync(0xFFFFFFFFu, l[t][j], 4);
                 l[t][j] += __shfl_xor_sync(0xFFFFFFFFu, l[t][j], 8);
                 l[t][j] += __shfl_xor_sync(0xFFFFFFFFu, l[t][j], 16);
-                if (lane < 4) stats[warp * S::HEADS + 8 * t + 2 * lane + j] = make_float2(m[t][j], l[t][j]);
+                if (lane < 4) stats[8 * t + 2 * lane + j] = make_float2(m[t][j], l[t][j]);
             }
-        __syncthreads();
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float top = -INFINITY;
+            for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-                for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w * S::HEADS + 8 * t + 2 * (lane & 3) + j].x);
-                const float f = exp2f(m[t][j] - (top == -INFINITY ? 0.f : top));
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s) o[t][s][j] *= f, o[t][s][j + 2] *= f;
+                for (int j = 0; j < 4; ++j) {
+                    const int d = 16 * s + (E4M3 ? 2 * (lane >> 2) + (j >> 1) : (lane >> 2) + 8 * (j >> 1));
+                    result[result_at<DP>(8 * t + 2 * (lane & 3) + (j & 1), d)] = o[t][s][j];
+                }
+        __syncwarp();
+        if (whole) {  // nobody else has any of it
+#pragma unroll 1
+            for (int h = 0; h < heads; ++h) {
+                const float f = inverse_sum(stats[h].y) * a.v_scale;
+#pragma unroll 1
+                for (int d0 = 0; d0 < DP; d0 += 128) {
+                    const int d = d0 + 4 * lane;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (d < a.dim) {
+                        v = *reinterpret_cast<const float4 *>(result + result_at<DP>(h, d));
+                        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                    }
+                    write_output(a, row, head0, h * a.dim + d, v, d < a.dim);
+                }
             }
-        const auto place = [&](int t, int s, int j) {  // of o[t][s][j] within a warp's results
-            const int r = lane >> 2;
-            const int d = 16 * s + (E4M3 ? 2 * r + (j >> 1) : r + 8 * (j >> 1));
-            return (8 * t + 2 * (lane & 3) + (j & 1)) * S::PITCH + d;
-        };
-        if (S::RED < W) {
-            if (warp >= S::RED) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) red[(warp - S::RED) * S::HEADS * S::PITCH + place(t, s, j)] = o[t][s][j];
-            }
-            __syncthreads();
-            if (warp < W - S::RED) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) o[t][s][j] += red[warp * S::HEADS * S::PITCH + place(t, s, j)];
-            }
+            if (WEIGHTS && lane < heads) a.norms[(int64_t)row * a.q_heads + head0 + lane] = make_float2(stats[lane].x, inverse_sum(stats[lane].y) * P::UP);
+            __syncwarp();
+            if (phase != MIDDLE && lane == 0) mine[phase == FIRST ? 0 : 1].n = 0;
         }
-        if (warp < S::RED) {
+    }
+    __syncthreads();
+
+    // ---- what the warps have of the same segment, together ----
+    // Entry 2w is warp w's first piece, 2w + 1 its last: in the order of the units.
+    const Entry entry = entries[lane < 2 * W ? lane : 0];
+    const bool exists = lane < 2 * W && entry.n > 0;
+    const uint32_t there = __ballot_sync(0xFFFFFFFFu, exists);
+    const uint32_t lower = there & ((1u << lane) - 1);
+    const int previous = lower ? 31 - __clz(lower) : 0;
+    const int previous_row = __shfl_sync(0xFFFFFFFFu, entry.row, previous), previous_segment = __shfl_sync(0xFFFFFFFFu, entry.segment, previous);
+    uint32_t starts = __ballot_sync(0xFFFFFFFFu, exists && (lower == 0 || previous_row != entry.row || previous_segment != entry.segment));
+    const auto result_of = [&](int i) {
+        return reinterpret_cast<const float *>(i & 1 ? smem + (i >> 1) * S::SLOTS * S::TILE : results + (i >> 1) * S::RESULT);
+    };
+    const auto members_of = [&](int i0) {  // the entries of the segment that begins with entry i0
+        const uint32_t from = ~((1u << i0) - 1), behind = starts & from & (from << 1);
+        return there & from & (behind ? (1u << (__ffs(behind) - 1)) - 1 : 0xFFFFFFFFu);
+    };
+    float *factors = reinterpret_cast<float *>(smem + S::RESULT);                    // [entry][head]: of its result
+    float2 *sums = reinterpret_cast<float2 *>(factors + 2 * W * S::HEADS);           // [first entry][head]: largest logit, sum of weights
+    {
+        const int i = threadIdx.x / S::HEADS, h = threadIdx.x % S::HEADS;
+        if (i < 2 * W && (there >> i & 1u)) {
+            const int i0 = 31 - __clz(starts & ((2u << i) - 1));
+            const uint32_t members = members_of(i0);
+            float2 st[2 * W];  // (all loads at once)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) red[warp * S::HEADS * S::PITCH + place(t, s, j)] = o[t][s][j];
-        }
-        __syncthreads();
-        const auto block_stats = [&](int h) {  // largest logit and sum over the block's warps
+            for (int k = 0; k < 2 * W; ++k) {
+                st[k] = make_float2(-INFINITY, 0.f);
+                if (members >> k & 1u) st[k] = reinterpret_cast<const float2 *>(result_of(k) + S::HEADS * DP)[h];
+            }
+            const float own_top = reinterpret_cast<const float2 *>(result_of(i) + S::HEADS * DP)[h].x;
             float top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) top = fmaxf(top, stats[w * S::HEADS + h].x);
+            for (int k = 0; k < 2 * W; ++k) top = fmaxf(top, st[k].x);
             const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < W; ++w) sum += stats[w * S::HEADS + h].y * exp2f(stats[w * S::HEADS + h].x - from);
-            return make_float2(top, sum);
-        };
-        const auto block_sum = [&](int h, int d) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < S::RED; ++w) {
-                const float4 x = *reinterpret_cast<const float4 *>(red + (w * S::HEADS + h) * S::PITCH + d);
-                v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
-            }
-            return v;
-        };
-
-        const int64_t segment_start = u0 + done - unit, segment_end = segment_start + seen.units;
-        const int n4 = heads * a.dim / 4;
-        if (piece == seen.units) {  // all of it
-            for (int e = threadIdx.x; e < (n4 + 31) / 32 * 32; e += S::THREADS) {
-                const bool there = e < n4;
+            for (int k = 0; k < 2 * W; ++k) sum += st[k].y * power2(st[k].x - from);
+            factors[threadIdx.x] = power2(own_top - from);
+            if (i == i0) sums[threadIdx.x] = make_float2(top, sum);
+        }
+    }
+    __syncthreads();
+    // a block has at most one segment that began before it and one that goes on behind it (or one that does both)
+    int n_unfinished = 0, unfinished0 = 0, unfinished1 = 0;  // those segments' first entries
+    int turn = warp;                                         // the warp's next head: the segments' heads go round
+#pragma unroll 1
+    for (uint32_t left = starts; left != 0; left &= left - 1) {
+        const int i0 = __ffs(left) - 1;
+        const uint32_t members = members_of(i0);
+        const Entry &f = entries[i0], &g = entries[31 - __clz(members)];
+        const bool whole = f.unit == 0 && g.unit + g.n == g.units;
+        if (!whole) {
+            if (n_unfinished++ == 0) unfinished0 = i0;
+            else unfinished1 = i0;
+        }
+        const int kv_head = a.tiles == 1 ? f.segment : f.segment / a.tiles, tile = f.segment - kv_head * a.tiles;
+        const int head0 = kv_head * a.group + tile * S::HEADS, heads = min(S::HEADS, a.group - tile * S::HEADS);
+        float *part = a.parts + (int64_t)(2 * blockIdx.x + (f.unit == 0 ? 1 : 0)) * S::PART;
+#pragma unroll 1
+        for (; turn < heads; turn += W) {  // a warp a head
+            const int h = turn;
+            const float2 st = sums[i0 * S::HEADS + h];
+            const float inv = inverse_sum(st.y), w = whole ? inv * a.v_scale : 1.f;
+#pragma unroll 1
+            for (int d0 = 0; d0 < DP; d0 += 128) {
+                const int d = d0 + 4 * lane;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (there) {
-                    const int h = 4 * e / a.dim;
-                    const float2 st = block_stats(h);
-                    const float f = inverse_sum(st.y) * a.v_scale;
-                    v = block_sum(h, 4 * e - h * a.dim);
-                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-                }
-                write_output(a, row, head0, 4 * e, v, there);
-            }
-            if (WEIGHTS) {
-                for (int h = threadIdx.x; h < heads; h += S::THREADS) {
-                    const float2 st = block_stats(h);
-                    a.norms[(int64_t)row * a.q_heads + head0 + h] = make_float2(st.x, inverse_sum(st.y) * P::UP);
-                }
-            }
-        } else {
-            float *part = a.parts + (int64_t)(2 * blockIdx.x + (unit == 0 ? 1 : 0)) * S::PART;
-            for (int e = threadIdx.x; e < n4; e += S::THREADS) {
-                const int h = 4 * e / a.dim, d = 4 * e - h * a.dim;
-                __stcg(reinterpret_cast<float4 *>(part + h * DP + d), block_sum(h, d));
-            }
-            for (int h = threadIdx.x; h < heads; h += S::THREADS) {
-                const float2 st = block_stats(h);
-                __stcg(part + S::HEADS * DP + h, st.x);
-                __stcg(part + S::HEADS * DP + S::HEADS + h, st.y);
-            }
-            __threadfence();
-            __syncthreads();
-            const int first = (int)(segment_start / per_block), last = (int)((segment_end - 1) / per_block);
-            if (threadIdx.x == 0) {
-                int *counter = a.counters + (int64_t)row * segments_row + segment;
-                is_last = atomicAdd(counter, 1) == last - first;
-                if (is_last) *counter = 0;  // for the next call
-            }
-            __syncthreads();
-            if (is_last) {
-                __threadfence();
-                const int n_parts = last - first + 1;
-                const auto part_of = [&](int i) { return a.parts + (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * S::PART; };
-                // factors of the parts, over the warps' results
-                float *factor = red;
-                for (int i = threadIdx.x; i < n_parts * heads; i += S::THREADS) {
-                    const int n = i / heads, h = i - n * heads;
-                    factor[n * S::HEADS + h] = __ldcg(part_of(n) + S::HEADS * DP + h);
-                }
-                __syncthreads();
-                for (int h = warp; h < heads; h += W) {
-                    float top = -INFINITY, sum = 0.f;
-                    for (int n = lane; n < n_parts; n += 32) top = fmaxf(top, factor[n * S::HEADS + h]);
+                if (d < a.dim) {
+#pragma unroll 1
+                    for (uint32_t b = members; b != 0;) {  // four at a time
+                        float c[4];
+                        float4 x[4];
 #pragma unroll
-                    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-                    const float from = top == -INFINITY ? 0.f : top;
-                    for (int n = lane; n < n_parts; n += 32) {
-                        const float f = exp2f(factor[n * S::HEADS + h] - from);
-                        sum += f * __ldcg(part_of(n) + S::HEADS * DP + S::HEADS + h);
-                        factor[n * S::HEADS + h] = f;
+                        for (int k = 0; k < 4; ++k) {
+                            const int i = b != 0 ? __ffs(b) - 1 : i0;
+                            c[k] = b != 0 ? factors[i * S::HEADS + h] : 0.f;
+                            x[k] = *reinterpret_cast<const float4 *>(result_of(i) + result_at<DP>(h, d));
+                            if (b == 0) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            b &= b - 1;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v = make_float4(v.x + c[k] * x[k].x, v.y + c[k] * x[k].y, v.z + c[k] * x[k].z, v.w + c[k] * x[k].w);
                     }
-#pragma unroll
-                    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, s);
-                    const float inv = inverse_sum(sum);
-                    for (int n = lane; n < n_parts; n += 32) factor[n * S::HEADS + h] *= inv * a.v_scale;
-                    if (WEIGHTS && lane == 0) a.norms[(int64_t)row * a.q_heads + head0 + h] = make_float2(top, inv * P::UP);
+                    v = make_float4(v.x * w, v.y * w, v.z * w, v.w * w);
+                    if (!whole) __stcg(reinterpret_cast<float4 *>(part + h * DP + d), v);
                 }
-                __syncthreads();
-                for (int e = threadIdx.x; e < (n4 + 31) / 32 * 32; e += S::THREADS) {
-                    const bool there = e < n4;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (there) {
-                        const int h = 4 * e / a.dim, d = 4 * e - h * a.dim;
+                if (whole) write_output(a, f.row, head0, h * a.dim + d, v, d < a.dim);
+            }
+            if (lane == 0 && !whole) __stcg(reinterpret_cast<float2 *>(part + S::HEADS * DP) + h, st);
+            if (WEIGHTS && lane == 0 && whole) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(st.x, inv * P::UP);
+        }
+        turn -= heads;
+    }
+
+    if (n_unfinished > 0) {
+        const auto blocks_of = [&](const Entry &f, int *first, int *n_parts) {
+            *first = first_block, *n_parts = parts_apart;
+            if (!apart) {
+                const uint32_t start = u0 + f.at - f.unit;
+                *first = start / per_block;
+                *n_parts = (start + f.units - 1) / per_block - *first + 1;
+            }
+        };
+        __syncthreads();  // all of the parts is written
+        if ((int)threadIdx.x < n_unfinished) {
+            const Entry &f = entries[threadIdx.x == 0 ? unfinished0 : unfinished1];
+            int first, n_parts, before;
+            blocks_of(f, &first, &n_parts);
+            int *counter = a.counters + (int64_t)f.row * segments_row + f.segment;
+            asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.s32 %0, [%1], 1;\n\tfence.acq_rel.gpu;" : "=r"(before) : "l"(counter) : "memory");
+            if (before == n_parts - 1) *counter = 0;  // for the next call
+            is_last[threadIdx.x] = before == n_parts - 1;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int k = 0; k < n_unfinished; ++k) {
+            if (!is_last[k]) continue;
+            const Entry &f = entries[k == 0 ? unfinished0 : unfinished1];
+            const int kv_head = a.tiles == 1 ? f.segment : f.segment / a.tiles, tile = f.segment - kv_head * a.tiles;
+            const int head0 = kv_head * a.group + tile * S::HEADS, heads = min(S::HEADS, a.group - tile * S::HEADS);
+            int first, n_parts;
+            blocks_of(f, &first, &n_parts);
+            // a block's part that begins a segment has a place of its own: the block may also have the end of the one before
+            const auto part_of = [&](int i) { return a.parts + (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * S::PART; };
+            const auto stat_of = [&](int i, int h) { return __ldcg(reinterpret_cast<const float2 *>(part_of(i) + S::HEADS * DP) + h); };
+#pragma unroll 1
+            for (int h = warp; h < heads; h += W) {  // a warp a head, a lane the weight of a part
+                float2 st = lane < n_parts ? stat_of(lane, h) : make_float2(-INFINITY, 0.f);
+                float top = st.x;
+#pragma unroll 1
+                for (int n = lane + 32; n < n_parts; n += 32) top = fmaxf(top, stat_of(n, h).x);
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, i));
+                const float from = top == -INFINITY ? 0.f : top;
+                float sum = 0.f;
+                float4 v[DP / 128 > 0 ? DP / 128 : 1];
+#pragma unroll
+                for (int c = 0; c < (DP + 127) / 128; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int n0 = 0; n0 < n_parts; n0 += 32) {
+                    if (n0 > 0) st = n0 + lane < n_parts ? stat_of(n0 + lane, h) : make_float2(-INFINITY, 0.f);
+                    const float mine_of = power2(st.x - from);
+                    sum += mine_of * st.y;
+                    const int n1 = min(32, n_parts - n0);
 #pragma unroll 8
-                        for (int n = 0; n < n_parts; ++n) {
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(n) + h * DP + d));
-                            const float f = factor[n * S::HEADS + h];
-                            v = make_float4(v.x + f * x.x, v.y + f * x.y, v.z + f * x.z, v.w + f * x.w);
+                    for (int n = 0; n < n1; ++n) {
+                        const float w = __shfl_sync(0xFFFFFFFFu, mine_of, n);
+#pragma unroll
+                        for (int c = 0; c < (DP + 127) / 128; ++c) {
+                            const int d = 128 * c + 4 * lane;
+                            if (d < a.dim) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(n0 + n) + h * DP + d));
+                                v[c] = make_float4(v[c].x + w * x.x, v[c].y + w * x.y, v[c].z + w * x.z, v[c].w + w * x.w);
+                            }
                         }
                     }
-                    write_output(a, row, head0, 4 * e, v, there);
                 }
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, i);
+                const float inv = inverse_sum(sum), w = inv * a.v_scale;
+#pragma unroll
+                for (int c = 0; c < (DP + 127) / 128; ++c) {
+                    const int d = 128 * c + 4 * lane;
+                    write_output(a, f.row, head0, h * a.dim + d, make_float4(v[c].x * w, v[c].y * w, v[c].z * w, v[c].w * w), d < a.dim);
+                }
+                if (WEIGHTS && lane == 0) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(top, inv * P::UP);
             }
         }
-        __syncthreads();  // the results' place is free for the next piece
+    }
 
-        done += piece;
-        unit += piece;
-        if (done < count && unit == seen.units) {
-            unit = 0;
-            if (++segment == segments_row) {
-                segment = 0;
-                do {
-                    seen = row_of(a, ++row);
-                } while (seen.units == 0);
-            }
-        }
+    // rows that see nothing get their zeros
+#pragma unroll 1
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const Row x = row_of(a, r);
+        if (x.seq < 0 || x.units > 0) continue;
+        const int n4 = a.q_heads * a.dim / 4;
+#pragma unroll 1
+        for (int e = threadIdx.x; e < (n4 + 31) / 32 * 32; e += S::THREADS)
+            write_output(a, r, 0, 4 * e, make_float4(0.f, 0.f, 0.f, 0.f), e < n4);
     }
 }
 
@@ -708,10 +963,13 @@ __global__ void __launch_bounds__(256) attention_weights_kernel(const AttnArgs a
     for (int64_t key = r.first + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; key < end; key += (int64_t)gridDim.x * blockDim.x) {
         const float *s = a.logits + (((int64_t)row * a.kv_heads + kv_head) * a.positions + key) * a.group;
         float given = 0.f;
-        for (int h = 0; h < a.group; ++h) given += exp2f(s[h] - norms[h].x) * norms[h].y;
+        for (int h = 0; h < a.group; ++h) given += power2(s[h] - norms[h].x) * norms[h].y;
         weights[((int64_t)row * a.kv_heads + kv_head) * weights_stride + key] += given;
     }
 }
+
+// More than eight query heads to a key head: sixteen in one pass over the keys, where the registers hold them.
+bool takes_16_heads(int64_t group, int64_t dim) { return group > 8 && dim <= 128; }
 
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -722,7 +980,8 @@ int workspace_of(int64_t rows, int64_t q_heads, const jq_kv_cache *c, bool weigh
     DeviceCaps caps;
     if (int rc = device_caps(&caps)) return rc;
     w->parts = rounded(JQ_PAGED_ATTENTION_COUNTERS(rows, q_heads));
-    const size_t part = 16 * 256 + 32;  // floats, the widest
+    const int64_t dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256, heads = takes_16_heads(q_heads / c->num_kv_heads, c->head_dim) ? 16 : 8;
+    const size_t part = heads * dim + 2 * heads;  // floats: Shape::PART of the instance that launch_for() takes
     w->norms = w->parts + rounded(2 * (size_t)caps.sm_count * part * sizeof(float));
     w->logits = w->norms + (weights ? rounded(sizeof(float2) * (size_t)rows * q_heads) : 0);
     w->total = w->logits + (weights ? rounded(sizeof(float) * (size_t)rows * q_heads * (size_t)(c->max_pages * c->page_size)) : 0);
@@ -730,13 +989,16 @@ int workspace_of(int64_t rows, int64_t q_heads, const jq_kv_cache *c, bool weigh
 }
 
 template <typename T, int DP, int NT, bool WEIGHTS>
-int launch_as(cudaStream_t st, AttnArgs &a, int blocks) {
+int launch_as(cudaStream_t st, AttnArgs &a, int sm_count) {
     using S = Shape<T, DP, NT>;
     const auto kernel = paged_attention_kernel<T, DP, NT, WEIGHTS>;
-    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::SMEM)) return rc;
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::SMEM, true)) return rc;
     a.tiles = (a.group + S::HEADS - 1) / S::HEADS;
+    const int64_t most = ((int64_t)a.positions + UNIT - 1) / UNIT * a.kv_heads * a.tiles * a.rows;
+    if (most > 0x7FFFFFFF)
+        return set_error(JQ_ERR_TOO_LARGE, "attention: %d rows of %d key heads with room for %d tokens are more than 2^31 units of %d", a.rows, a.kv_heads, a.positions, UNIT);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = dim3((unsigned)sm_count);
     cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
@@ -750,17 +1012,17 @@ int launch_as(cudaStream_t st, AttnArgs &a, int blocks) {
 }
 
 template <typename T, bool WEIGHTS>
-int launch_for(cudaStream_t st, AttnArgs &a, int blocks) {
-    if (a.dim > 128) return launch_as<T, 256, 1, WEIGHTS>(st, a, blocks);
-    if (a.group > 8) return a.dim > 64 ? launch_as<T, 128, 2, WEIGHTS>(st, a, blocks) : launch_as<T, 64, 2, WEIGHTS>(st, a, blocks);
-    return a.dim > 64 ? launch_as<T, 128, 1, WEIGHTS>(st, a, blocks) : launch_as<T, 64, 1, WEIGHTS>(st, a, blocks);
+int launch_for(cudaStream_t st, AttnArgs &a, int sm_count) {
+    if (a.dim > 128) return launch_as<T, 256, 1, WEIGHTS>(st, a, sm_count);
+    if (takes_16_heads(a.group, a.dim)) return a.dim > 64 ? launch_as<T, 128, 2, WEIGHTS>(st, a, sm_count) : launch_as<T, 64, 2, WEIGHTS>(st, a, sm_count);
+    return a.dim > 64 ? launch_as<T, 128, 1, WEIGHTS>(st, a, sm_count) : launch_as<T, 64, 1, WEIGHTS>(st, a, sm_count);
 }
 
 template <bool WEIGHTS>
-int launch_type(cudaStream_t st, AttnArgs &a, int type, int blocks) {
-    if (type == JQ_KV_F16) return launch_for<KvF16, WEIGHTS>(st, a, blocks);
-    if (type == JQ_KV_BF16) return launch_for<KvBf16, WEIGHTS>(st, a, blocks);
-    return launch_for<KvE4m3, WEIGHTS>(st, a, blocks);
+int launch_type(cudaStream_t st, AttnArgs &a, int type, int sm_count) {
+    if (type == JQ_KV_F16) return launch_for<KvF16, WEIGHTS>(st, a, sm_count);
+    if (type == JQ_KV_BF16) return launch_for<KvBf16, WEIGHTS>(st, a, sm_count);
+    return launch_for<KvE4m3, WEIGHTS>(st, a, sm_count);
 }
 
 int check_heads(int64_t rows, int64_t q_heads, const jq_kv_cache *c) {
@@ -823,14 +1085,15 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
         return set_error(JQ_ERR_INVALID_ARG, "attention: a workspace of %zu bytes is needed, %zu given", w.total, ws_bytes);
     DeviceCaps caps;
     if (int rc = device_caps(&caps)) return rc;
-    const int blocks = caps.sm_count < MAX_BLOCKS ? caps.sm_count : MAX_BLOCKS;
     a.q = d_q, a.q_row = q_stride_row, a.q_head = q_stride_head;
     a.k = static_cast<const char *>(cache->d_k), a.v = static_cast<const char *>(cache->d_v);
     a.lens = d_lens, a.seqs = d_seqs, a.out = d_out, a.xq = static_cast<uint8_t *>(d_xq);
-    a.scale_log2 = (float)((double)scale * cache->k_scale * 1.4426950408889634);
+    a.scale_log2 = std::fmax((float)(std::fabs((double)scale) * cache->k_scale * 1.4426950408889634), 1e-30f);  // (0: all logits vanish)
+    a.negative = scale < 0.f;
     a.v_scale = cache->v_scale;
     a.rows = (int)num_rows, a.q_heads = (int)num_q_heads, a.kv_heads = (int)cache->num_kv_heads, a.group = a.q_heads / a.kv_heads, a.dim = (int)dim;
-    a.positions = cache->max_pages * cache->page_size;
+    a.positions = (int)(cache->max_pages * cache->page_size);
+    a.grouped = cache->page_size % UNIT == 0;
     a.window = window >= a.positions ? 0 : (int)window;
     a.n_super = (int)(num_q_heads * dim / SUPER), a.order = order, a.s_mode = s_mode;
     char *ws = static_cast<char *>(d_ws);
@@ -840,10 +1103,10 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
     a.logits = reinterpret_cast<float *>(ws + w.logits);
     a.fault = device_fault_ptr();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (d_weights == nullptr) return launch_type<false>(st, a, cache->type, blocks);
-    if (int rc = launch_type<true>(st, a, cache->type, blocks)) return rc;
+    if (d_weights == nullptr) return launch_type<false>(st, a, cache->type, caps.sm_count);
+    if (int rc = launch_type<true>(st, a, cache->type, caps.sm_count)) return rc;
     if (a.positions == 0) return JQ_OK;
-    int64_t across = (a.positions + 255) / 256;
+    int across = (a.positions + 255) / 256;
     if (across > 64) across = 64;  // a block walks on where sequences are longer
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)across, (unsigned)a.kv_heads, (unsigned)num_rows);

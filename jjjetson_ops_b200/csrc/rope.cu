@@ -294,11 +294,7 @@ int check_kv_cache(const jq_kv_cache *c, KvIndex *ix) {
     ix->num_seqs = (int32_t)c->num_seqs;
     ix->max_pages = (int32_t)c->max_pages;
     ix->num_pages = (int32_t)c->num_pages;
-    ix->page_size = (int32_t)c->page_size;
-    ix->page_shift = -1;
-    for (int s = 0; s < 31; ++s) {
-        if (c->page_size == (int64_t)1 << s) ix->page_shift = s;
-    }
+    kv_set_page_size(*ix, (int32_t)c->page_size);
     return JQ_OK;
 }
 
