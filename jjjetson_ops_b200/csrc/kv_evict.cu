@@ -7,7 +7,7 @@
 // SM to a head.  What bounds it is latency: three histograms one after the other.
 //
 // Moving: bound by bytes, each kept row read and written once.  Into other pages all rows move at once.  Within the same pages a row may only
-// be overwritten after it was read: a block has a column of 64 bytes of all rows of a head to itself and takes the rows in their
+// be overwritten after it was read: a block has a column of 32 bytes of all rows of a head to itself and takes the rows in their
 // order, a tile of loads before the tile's stores (a row never moves back, so later tiles read behind all earlier stores).
 #include <cooperative_groups.h>
 
@@ -19,11 +19,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SELECT_THREADS = 512;
+constexpr int SELECT_THREADS = 1024;
 constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
+static_assert(SELECT_WARPS == 32, "a lane for every warp");
 constexpr int DIGITS = 3;
-constexpr int BINS = 2048;  // four per thread
+constexpr int BINS = 2048;
+constexpr int BINS_PER_THREAD = BINS / SELECT_THREADS;
 constexpr int64_t MAX_SLICE = 48 * 1024;  // weights of one block
 
 struct EvictArgs {
@@ -86,31 +88,50 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
 
     const int slice = ((n + parts - 1) / parts + 31) / 32 * 32;
     const int first = min(n, part * slice), mine = min(n, first + slice) - first;
-    for (int i = threadIdx.x; i < mine; i += SELECT_THREADS) w[i] = from[first + i];
-    for (int i = threadIdx.x; i < DIGITS * BINS; i += SELECT_THREADS) (&bins[0][0])[i] = 0;
+    for (int i = threadIdx.x; i < DIGITS * BINS / 4; i += SELECT_THREADS) reinterpret_cast<uint4 *>(&bins[0][0])[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-
-    // the weight of the last token that stays, of those that are not kept anyway
     const int low = a.sinks, high = n - a.recent;  // candidates
     const int c0 = max(low - first, 0), c1 = min(high - first, mine);
     uint32_t left = (uint32_t)(a.keep - a.sinks - a.recent), prefix = 0;
-    constexpr int SHIFT[DIGITS] = {21, 10, 0};
+    // the slice into shared memory, eight loads of a thread at a time, and into the first histogram
+    for (int i0 = threadIdx.x; i0 < mine; i0 += 8 * SELECT_THREADS) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u * SELECT_THREADS;
+            x[u] = i < mine ? from[first + i] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u * SELECT_THREADS;
+            if (i < mine) w[i] = x[u];
+            if (i >= c0 && i < c1) atomicAdd(&bins[0][key_of(x[u]) >> 21], 1u);
+        }
+    }
+
+    // the weight of the last token that stays, of those that are not kept anyway
+    const auto everybody = [&]() {
+        if (parts > 1) cluster.sync();
+        else __syncthreads();
+    };
     if (left > 0) {
 #pragma unroll
         for (int digit = 0; digit < DIGITS; ++digit) {
-            for (int i = c0 + (int)threadIdx.x; i < c1; i += SELECT_THREADS) {
-                const uint32_t key = key_of(w[i]);
-                if (digit == 0 || key >> (digit == 1 ? 21 : 10) == prefix)
-                    atomicAdd(&bins[digit][digit == 2 ? key & 1023u : key >> SHIFT[digit] & (BINS - 1)], 1u);
+            if (digit > 0) {
+                for (int i = c0 + (int)threadIdx.x; i < c1; i += SELECT_THREADS) {
+                    const uint32_t key = key_of(w[i]);
+                    if (key >> (digit == 1 ? 21 : 10) == prefix) atomicAdd(&bins[digit][digit == 1 ? key >> 10 & (BINS - 1) : key & 1023u], 1u);
+                }
             }
-            cluster.sync();
-            uint4 sum = make_uint4(0, 0, 0, 0);  // bins 4t .. 4t + 3
+            everybody();
+            uint2 sum = make_uint2(0, 0);  // this thread's two bins, over the blocks
+#pragma unroll 4
             for (int p = 0; p < parts; ++p) {
-                const uint4 x = reinterpret_cast<const uint4 *>(cluster.map_shared_rank(&bins[digit][0], p))[threadIdx.x];
-                sum = make_uint4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+                const uint2 x = reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&bins[digit][0], p))[threadIdx.x];
+                sum = make_uint2(sum.x + x.x, sum.y + x.y);
             }
             // how many lie in higher bins
-            const uint32_t own = sum.x + sum.y + sum.z + sum.w;
+            const uint32_t own = sum.x + sum.y;
             uint32_t up = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -119,14 +140,12 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
             }
             if (lane == 0) sums[warp] = up;
             __syncthreads();
-            uint32_t above = up - own;
-            for (int v = warp + 1; v < SELECT_WARPS; ++v) above += sums[v];
+            const uint32_t behind = __reduce_add_sync(0xFFFFFFFFu, lane > warp ? sums[lane] : 0u);
+            uint32_t above = up - own + behind;
             if (above < left && left <= above + own) {
-                const uint32_t b[4] = {sum.x, sum.y, sum.z, sum.w};
-                int i = 3;
-                while (above + b[i] < left) above += b[i--];
-                found_bin = 4 * threadIdx.x + i;
-                found_left = left - above;
+                const bool upper = left <= above + sum.y;
+                found_bin = BINS_PER_THREAD * threadIdx.x + (upper ? 1 : 0);
+                found_left = left - above - (upper ? 0 : sum.y);
             }
             __syncthreads();
             left = found_left;
@@ -134,7 +153,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
         }
     } else {
         prefix = 0xFFFFFFFFu;  // above every key
-        cluster.sync();        // all slices are loaded before weights are written
+        everybody();           // all slices are loaded before weights are written
     }
     const uint32_t last_key = prefix;
     const int of_equal = (int)left;  // so many of those with the last weight stay, the first ones
@@ -157,18 +176,19 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
     }
     if (lane == 0) warp_counts[warp] = count;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Counts all = {0, 0};
-        for (int v = 0; v < SELECT_WARPS; ++v) all.above += warp_counts[v].above, all.equal += warp_counts[v].equal;
-        block_counts = all;
+    const Counts of_lane = warp_counts[lane];
+    if (parts > 1) {
+        if (warp == 0) {
+            const Counts all = {__reduce_add_sync(0xFFFFFFFFu, of_lane.above), __reduce_add_sync(0xFFFFFFFFu, of_lane.equal)};
+            if (lane == 0) block_counts = all;
+        }
+        cluster.sync();
     }
-    cluster.sync();
-    Counts before = {0, 0};
+    Counts before = {__reduce_add_sync(0xFFFFFFFFu, lane < warp ? of_lane.above : 0), __reduce_add_sync(0xFFFFFFFFu, lane < warp ? of_lane.equal : 0)};
     for (int p = 0; p < part; ++p) {
         const Counts c = *cluster.map_shared_rank(&block_counts, p);
         before.above += c.above, before.equal += c.equal;
     }
-    for (int v = 0; v < warp; ++v) before.above += warp_counts[v].above, before.equal += warp_counts[v].equal;
     for (int i = s0 + lane; i - lane < s1; i += 32) {
         bool above, equal;
         flags(i, &above, &equal);
@@ -184,7 +204,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
         before.equal += __popc(same);
     }
     for (int64_t i = stays + thread; i < a.max_len; i += threads) new_w[i] = 0.f;
-    cluster.sync();  // no block ends while another reads its counts
+    if (parts > 1) cluster.sync();  // no block ends while another reads its counts
 }
 
 __device__ __forceinline__ int64_t place_of(const KvIndex &ix, int seq, int token, int *fault) {
@@ -234,9 +254,9 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictArg
 }
 
 constexpr int SHIFT_THREADS = 512;
-constexpr int COLUMN = 64;  // bytes
+constexpr int COLUMN = 32;  // bytes
 
-// Within the same pages: four threads have a row's 64 bytes.
+// Within the same pages: two threads have a row's 32 bytes.
 template <typename E>
 __global__ void __launch_bounds__(SHIFT_THREADS) evict_shift_kernel(const EvictArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -246,17 +266,17 @@ __global__ void __launch_bounds__(SHIFT_THREADS) evict_shift_kernel(const EvictA
     const bool values = (int)blockIdx.x >= columns;
     if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) write_length(a, seq);
     char *rows = values ? a.v : a.k;
-    const int chunk = ((int)blockIdx.x - (values ? columns : 0)) * COLUMN + (threadIdx.x & 3) * 16;
+    const int chunk = ((int)blockIdx.x - (values ? columns : 0)) * COLUMN + (threadIdx.x & 1) * 16;
     const bool inside = chunk < a.row_bytes;
     const int64_t column = (int64_t)head * a.ix.stride_head * (int)sizeof(E) + chunk;
     const int32_t *kept = a.kept + ((int64_t)seq * a.kv_heads + head) * a.keep;
-    constexpr int ROWS = SHIFT_THREADS / 4;
+    constexpr int ROWS = SHIFT_THREADS / 2;
     for (int j0 = 0; j0 < a.keep && kept[j0] >= 0; j0 += ROWS * MOVE_AT_ONCE) {
         uint4 x[MOVE_AT_ONCE];
         int64_t to[MOVE_AT_ONCE];
 #pragma unroll
         for (int u = 0; u < MOVE_AT_ONCE; ++u) {
-            const int j = j0 + u * ROWS + (threadIdx.x >> 2);
+            const int j = j0 + u * ROWS + (threadIdx.x >> 1);
             to[u] = -1;
             if (j >= a.keep || !inside) continue;
             const int i = kept[j];

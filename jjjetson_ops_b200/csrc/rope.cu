@@ -13,7 +13,7 @@ namespace jq {
 namespace {
 
 constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_MAX_ROWS = 4;     // rows of a block: as many angles as threads for 128-wide heads
+constexpr int ROPE_MAX_ROWS = 2;     // of a block
 
 struct RopeArgs {
     const float *x;
@@ -88,15 +88,29 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
     at.first = INTERLEAVED || !at.turns ? 2 * W * u : W * u;
     at.second = INTERLEAVED || !at.turns ? at.first + W : a.half + W * u;
 
-    // the first head's elements are on their way while the angles are computed
-    float p[W], q[W];
-    int head = head0 + lane_head;
-    const auto load = [&](int row, int h) {
-        const float *x = a.x + (int64_t)(row0 + row) * a.x_row + (int64_t)h * a.x_head;
-        load_floats<W>(p, x + at.first);
-        load_floats<W>(q, x + at.second);
+    // a head's elements are asked for while the one before it is worked on; the first one's while the angles are computed
+    float next_p[W], next_q[W];
+    int next_row = 0, next_head = head0 + lane_head;
+    const float *next_x = a.x + (int64_t)row0 * a.x_row + (int64_t)next_head * a.x_head;
+    const auto load = [&]() {
+        if (INTERLEAVED && W >= 2) {
+            float y[2 * W];
+            load_floats<2 * W>(y, next_x + at.first);
+#pragma unroll
+            for (int i = 0; i < W; ++i) next_p[i] = y[i], next_q[i] = y[W + i];
+        } else {
+            load_floats<W>(next_p, next_x + at.first);
+            load_floats<W>(next_q, next_x + at.second);
+        }
+        next_head += step;
+        next_x += step * a.x_head;
+        if (next_head >= head1) {
+            ++next_row;
+            next_head = head0 + lane_head;
+            next_x = a.x + (int64_t)(row0 + next_row) * a.x_row + (int64_t)next_head * a.x_head;
+        }
     };
-    if (head < head1) load(0, head);
+    if (next_head < head1) load();
 
     for (int i = threadIdx.x; CACHE && head1 > a.heads && i < rows; i += blockDim.x) {
         const int row = row0 + i;
@@ -125,8 +139,11 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
                 c[i] = t.x, s[i] = t.y;
             }
         }
-        for (head = head0 + lane_head; head < head1; head += step) {
-            if (row != 0 || head != head0 + lane_head) load(row, head);
+        for (int head = head0 + lane_head; head < head1; head += step) {
+            float p[W], q[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) p[i] = next_p[i], q[i] = next_q[i];
+            if (next_row < rows) load();
             const bool is_value = CACHE && head >= a.heads + a.kv_heads;
             if (at.turns && !is_value) {
                 float y[2 * W];
@@ -151,8 +168,15 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
             }
             if (!CACHE || head < a.heads) {
                 float *y = a.out + (int64_t)(row0 + row) * a.out_row + (int64_t)head * a.out_head;
-                store_floats<W>(y + at.first, p);
-                store_floats<W>(y + at.second, q);
+                if (INTERLEAVED && W >= 2) {
+                    float both[2 * W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) both[i] = p[i], both[W + i] = q[i];
+                    store_floats<2 * W>(y + at.first, both);
+                } else {
+                    store_floats<W>(y + at.first, p);
+                    store_floats<W>(y + at.second, q);
+                }
             }
             if constexpr (CACHE) {
                 if (head >= a.heads && place[row] >= 0) {
@@ -192,8 +216,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
 int pairs_per_thread(const RopeArgs &a, int rotary_dim, int interleaved) {
     for (int w = 4; w > 1; w >>= 1) {
         if (rotary_dim % (2 * w) != 0 || (a.dim - rotary_dim) % (2 * w) != 0) continue;
-        // (both layouts load W floats at a time: a group of interleaved pairs is two loads of W)
-        const uintptr_t mask = (w == 4 ? 16 : 8) - 1;
+        const uintptr_t mask = (w == 4 || interleaved ? 16 : 8) - 1;
         const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)(a.x_row * 4) | (uintptr_t)(a.x_head * 4) |
                                (uintptr_t)(a.out_row * 4) | (uintptr_t)(a.out_head * 4);
         if ((bits & mask) != 0) continue;
@@ -215,7 +238,9 @@ int launch_rope_as(cudaStream_t st, RopeArgs &a, int rotary_dim) {
     // Few rows: a block per row and as many heads as it takes at once.  Many: a block takes some rows, and all their heads.
     const int64_t blocks_per_row = (all_heads + used - 1) / used;
     const bool few = a.rows * blocks_per_row <= 4 * (int64_t)caps.sm_count;
-    a.rows_per_block = few ? 1 : ROPE_MAX_ROWS;
+    // (two rows where that leaves every SM its eight blocks.  us with four rows, two, one: 8192 rows of 64 x 128 85.4, 83.7, 84.0; 4097 rows
+    // of 32 + 2 x 8 heads into a cache 34.4, 31.4, 33.3; 2049 of 25 x 80 10.2, 9.4, 9.1)
+    a.rows_per_block = few || a.rows < ROPE_MAX_ROWS * 8 * (int64_t)caps.sm_count ? 1 : ROPE_MAX_ROWS;
     a.heads_per_block_y = few ? used : all_heads;
     const size_t smem = sizeof(float2) * (size_t)a.rows_per_block * a.half;
     cudaLaunchConfig_t cfg = {};
