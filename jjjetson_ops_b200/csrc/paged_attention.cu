@@ -26,6 +26,10 @@ namespace jq {
 namespace {
 
 constexpr int UNIT = 16;          // keys; what the work is divided by
+// What a warp spends on the beginning of a segment (its queries, and what it had of the one before into shared memory), in units: stretches are
+// equal with this counted in.  Without it the warps of a block that had one segment more were done 6 us later (16 sequences of up to
+// 2500 tokens, 32 key heads).
+constexpr int BEGIN = 5;
 constexpr int STEP = 2;           // units that a warp takes at a time: two tiles of 16 rows for the tensor cores
 constexpr int SMEM_BYTES = 227 * 1024;
 
@@ -132,7 +136,7 @@ __device__ __forceinline__ float power2(float x) {
 // One warp's part of a piece, by its place in the order: where the piece lies, and where the part does.
 struct Entry {
     int row, segment, unit, n, units;  // units [unit, unit + n) of the row's
-    int at;                            // where they lie in the block's stretch
+    int start;                         // where the segment begins, from the block's beginning on
 };
 
 // Shapes of one instance.
@@ -150,7 +154,7 @@ struct Shape {
     static constexpr int KEYS = STEP * UNIT;
     static constexpr int TILE = KEYS * ROW;         // keys, or values, of a step
     static constexpr int RESULT = HEADS * DP * 4 + HEADS * 8;  // a warp's result: sums, then per head the largest logit and the sum of weights
-    static constexpr int FIXED = WARPS * (RESULT + 2 * (int)sizeof(Entry) + 32) + 16;
+    static constexpr int FIXED = WARPS * (RESULT + 2 * (int)sizeof(Entry) + 32) + 32;
     static constexpr int FIT = (SMEM_BYTES - FIXED) / (WARPS * TILE);
     static constexpr int SLOTS = FIT < 6 ? FIT : 6;
     static constexpr int RING = WARPS * SLOTS * TILE;
@@ -277,6 +281,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     // ---- the block's stretch ----
     Row own = {-1, 0, 0, 0, 0};  // the row of this lane's number
     if (lane < a.rows) own = row_of(a, lane);
+    const auto weight_of = [&](const Row &r) { return r.units > 0 ? r.units + BEGIN : 0; };  // of one of its segments
     uint32_t total = own.units * segments_row, segments = own.units > 0 ? segments_row : 0;
 #pragma unroll 1
     for (int r = lane + 32; r < a.rows; r += 32) {
@@ -289,6 +294,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     // Few segments: each gets blocks of its own, so that a block has one segment to put together; at most an eighth of the blocks stay
     // idle.  Many: equal stretches.
     const bool apart = segments * 8 <= gridDim.x;
+    if (!apart) total += segments * BEGIN;
     uint32_t per_block = apart ? (total + gridDim.x - segments - 1) / (gridDim.x - segments) : (total + gridDim.x - 1) / gridDim.x;
     if (per_block < S::LEAST) per_block = S::LEAST;
     const uint32_t u0 = blockIdx.x * per_block;  // (not apart)
@@ -320,69 +326,79 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
         }
         piece.unit += warp * STEP;
         a1 = max(0, count - warp * STEP);
-    } else if (u0 < total) {
-        count = min(per_block, total - u0);
-        a0 = warp * count / W, a1 = (warp + 1) * count / W;
-        if (a0 < a1) {
-            uint32_t within;
-            piece.r = find_row(a, own, u0 + a0, [&](const Row &r) { return segments_row * r.units; }, &within);
-            piece.row = row_at(a, own, piece.r);
-            piece.segment = within / piece.row.units;
-            piece.unit = within - piece.segment * piece.row.units;
-        }
     }
 
     // ---- the warp's pieces: first those that begin and end with it, then the one that began before, then the last ----
     // (so that what it has of the first piece stays where the others' results were turned around)
     Entry *mine = entries + 2 * warp;  // [0]: the first piece where others follow, [1]: the last; n = 0: none
-    int middle = 0;                    // units of the pieces between the two
-    {
-        const int n = a1 - a0;
-        Entry first = {piece.r, piece.segment, piece.unit, n > 0 ? min(n, piece.row.units - piece.unit) : 0, piece.row.units, a0}, last = first;
-        if (first.n < n) {
-            uint32_t within;
-            last.row = find_row(a, own, u0 + a1 - 1, [&](const Row &r) { return segments_row * r.units; }, &within);
-            last.units = row_at(a, own, last.row).units;
-            last.segment = within / last.units;
-            last.unit = 0;
-            last.n = within - last.segment * last.units + 1;
-            last.at = a1 - last.n;
-            middle = n - first.n - last.n;
+    Entry first_piece = {piece.r, piece.segment, piece.unit, a1, piece.row.units, 0}, last_piece = first_piece;
+    first_piece.n = 0;
+    if (!apart && u0 < total) {
+        count = min(per_block, total - u0);
+        a0 = warp * count / W, a1 = (warp + 1) * count / W;
+        if (a0 < a1) {
+            const auto find = [&](int at, Entry &e) {  // the segment at `at`, and which of its units begins there
+                uint32_t within;
+                e.row = find_row(a, own, u0 + at, [&](const Row &r) { return segments_row * weight_of(r); }, &within);
+                e.units = __shfl_sync(0xFFFFFFFFu, own.units, e.row & 31);
+                if (e.row >= 32) e.units = row_of(a, e.row).units;
+                e.segment = within / (e.units + BEGIN);
+                e.unit = within - e.segment * (e.units + BEGIN);
+                e.start = at - e.unit;
+                e.unit = max(0, e.unit - BEGIN);
+            };
+            find(a0, first_piece);
+            find(a1, last_piece);  // (at the call's end: nonsense, and not looked at)
+            const bool to_the_end = u0 + a1 >= total;
+            if (!to_the_end && last_piece.row == first_piece.row && last_piece.segment == first_piece.segment) {
+                first_piece.n = last_piece.unit - first_piece.unit;
+                last_piece = first_piece;
+                first_piece.n = 0;
+            } else {
+                first_piece.n = first_piece.units - first_piece.unit;
+                last_piece.n = to_the_end ? 0 : last_piece.unit;
+                if (to_the_end) last_piece.row = a.rows;
+                last_piece.unit = 0;
+            }
         } else {
-            first.n = 0;
+            last_piece.n = 0;
         }
-        if (lane == 0) mine[0] = first, mine[1] = last;
-        __syncwarp();
     }
-    const bool any = a0 < a1;
+    if (lane == 0) mine[0] = first_piece, mine[1] = last_piece;
+    __syncwarp();
+    const bool any = first_piece.n > 0 || last_piece.n > 0;
     // A walk over the pieces; `row` and the others of the piece are what the walker needs of it.
     enum { MIDDLE, FIRST, LAST, DONE };
     struct Walk {
         Row row;
         int r, segment, unit, n;  // units left of the piece, from `unit` on
-        int phase, middle;
+        int phase;
     };
     const auto next_piece = [&](Walk &w) {
-        if (w.phase == MIDDLE && w.middle > 0) {  // the next segment, all of it
+        if (w.phase == MIDDLE) {  // the next segment, all of it, if it is not the one that the last piece is of
             if (++w.segment == segments_row) {
                 w.segment = 0;
 #pragma unroll 1
                 do {
-                    w.row = row_of(a, ++w.r);
-                } while (w.row.units == 0);
+                    ++w.r;
+                    if (w.r < a.rows) w.row = row_of(a, w.r);
+                } while (w.r < a.rows && w.row.units == 0);
             }
             w.unit = 0;
             w.n = w.row.units;
-            w.middle -= w.n;
-        } else if (++w.phase != DONE) {
+            if (w.r < a.rows && (w.r != mine[1].row || w.segment != mine[1].segment)) return;
+        }
+        ++w.phase;
+        if (w.phase == LAST && mine[1].n == 0) w.phase = DONE;
+        if (w.phase != DONE) {
             const Entry &e = mine[w.phase == FIRST ? 0 : 1];
             w.r = e.row, w.segment = e.segment, w.unit = e.unit, w.n = e.n;
             w.row = row_of(a, w.r);
         }
     };
     Walk at, next;  // what is computed, and what is copied
-    at.row = piece.row, at.r = piece.r, at.segment = piece.segment, at.middle = middle;
-    at.phase = !any ? LAST : mine[0].n > 0 ? MIDDLE : FIRST;  // (the phase before that of the first piece to take)
+    at.row = row_at(a, own, any ? first_piece.row : 0), at.r = first_piece.row, at.segment = first_piece.segment;
+    at.phase = !any ? LAST : first_piece.n > 0 ? MIDDLE : FIRST;  // (the phase before that of the first piece to take)
     next_piece(at);
     next = at;
 
@@ -802,19 +818,15 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
         if (i < 2 * W && (there >> i & 1u)) {
             const int i0 = 31 - __clz(starts & ((2u << i) - 1));
             const uint32_t members = members_of(i0);
-            float2 st[2 * W];  // (all loads at once)
-#pragma unroll
-            for (int k = 0; k < 2 * W; ++k) {
-                st[k] = make_float2(-INFINITY, 0.f);
-                if (members >> k & 1u) st[k] = reinterpret_cast<const float2 *>(result_of(k) + S::HEADS * DP)[h];
-            }
-            const float own_top = reinterpret_cast<const float2 *>(result_of(i) + S::HEADS * DP)[h].x;
+            // (loops that stay loops: instructions that are executed once come from the second-level cache, a line of eight at a time)
+            const auto stat = [&](uint32_t b) { return reinterpret_cast<const float2 *>(result_of(__ffs(b) - 1) + S::HEADS * DP)[h]; };
+            const float own_top = stat(1u << i).x;
             float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 2 * W; ++k) top = fmaxf(top, st[k].x);
+#pragma unroll 1
+            for (uint32_t b = members; b != 0; b &= b - 1) top = fmaxf(top, stat(b).x);
             const float from = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int k = 0; k < 2 * W; ++k) sum += st[k].y * power2(st[k].x - from);
+#pragma unroll 1
+            for (uint32_t b = members; b != 0; b &= b - 1) sum += stat(b).y * power2(stat(b).x - from);
             factors[threadIdx.x] = power2(own_top - from);
             if (i == i0) sums[threadIdx.x] = make_float2(top, sum);
         }
@@ -873,78 +885,94 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     }
 
     if (n_unfinished > 0) {
-        const auto blocks_of = [&](const Entry &f, int *first, int *n_parts) {
-            *first = first_block, *n_parts = parts_apart;
-            if (!apart) {
-                const uint32_t start = u0 + f.at - f.unit;
-                *first = start / per_block;
-                *n_parts = (start + f.units - 1) / per_block - *first + 1;
-            }
-        };
+        int *part_first = is_last + 2, *part_count = is_last + 4;  // of the two segments: the first of their blocks, and how many
         __syncthreads();  // all of the parts is written
         if ((int)threadIdx.x < n_unfinished) {
             const Entry &f = entries[threadIdx.x == 0 ? unfinished0 : unfinished1];
-            int first, n_parts, before;
-            blocks_of(f, &first, &n_parts);
+            int first = first_block, n_parts = parts_apart, before;
+            if (!apart) {
+                const uint32_t start = u0 + f.start + BEGIN;  // of its units
+                first = start / per_block;
+                n_parts = (start + f.units - 1) / per_block - first + 1;
+            }
+            part_first[threadIdx.x] = first, part_count[threadIdx.x] = n_parts;
             int *counter = a.counters + (int64_t)f.row * segments_row + f.segment;
             asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.s32 %0, [%1], 1;\n\tfence.acq_rel.gpu;" : "=r"(before) : "l"(counter) : "memory");
             if (before == n_parts - 1) *counter = 0;  // for the next call
             is_last[threadIdx.x] = before == n_parts - 1;
         }
         __syncthreads();
+        // a warp a head of one of the two, a lane the weight of a part
+        const int each = min(S::HEADS, a.group);
 #pragma unroll 1
-        for (int k = 0; k < n_unfinished; ++k) {
+        for (int turn = warp; turn < n_unfinished * each; turn += W) {
+            const int k = turn >= each, h = turn - k * each;
             if (!is_last[k]) continue;
             const Entry &f = entries[k == 0 ? unfinished0 : unfinished1];
             const int kv_head = a.tiles == 1 ? f.segment : f.segment / a.tiles, tile = f.segment - kv_head * a.tiles;
             const int head0 = kv_head * a.group + tile * S::HEADS, heads = min(S::HEADS, a.group - tile * S::HEADS);
-            int first, n_parts;
-            blocks_of(f, &first, &n_parts);
+            if (h >= heads) continue;
+            const int first = part_first[k], n_parts = part_count[k];
             // a block's part that begins a segment has a place of its own: the block may also have the end of the one before
-            const auto part_of = [&](int i) { return a.parts + (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * S::PART; };
-            const auto stat_of = [&](int i, int h) { return __ldcg(reinterpret_cast<const float2 *>(part_of(i) + S::HEADS * DP) + h); };
-#pragma unroll 1
-            for (int h = warp; h < heads; h += W) {  // a warp a head, a lane the weight of a part
-                float2 st = lane < n_parts ? stat_of(lane, h) : make_float2(-INFINITY, 0.f);
-                float top = st.x;
-#pragma unroll 1
-                for (int n = lane + 32; n < n_parts; n += 32) top = fmaxf(top, stat_of(n, h).x);
+            const auto part_of = [&](int i) { return a.parts + (2 * (first + i) + (i == 0 ? 1 : 0)) * S::PART; };
+            const auto stat_of = [&](int i) { return __ldcg(reinterpret_cast<const float2 *>(part_of(i) + S::HEADS * DP) + h); };
+            constexpr int ACROSS = (DP + 127) / 128;
+            const auto sums_of = [&](int i, int c) {
+                const int d = 128 * c + 4 * lane;
+                return d < a.dim ? __ldcg(reinterpret_cast<const float4 *>(part_of(i) + h * DP + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            constexpr int EARLY = 4;  // parts whose sums are on their way while the weights are made
+            float4 early[EARLY][ACROSS];
+            float2 st = lane < n_parts ? stat_of(lane) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, i));
-                const float from = top == -INFINITY ? 0.f : top;
-                float sum = 0.f;
-                float4 v[DP / 128 > 0 ? DP / 128 : 1];
+            for (int n = 0; n < EARLY; ++n)
 #pragma unroll
-                for (int c = 0; c < (DP + 127) / 128; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int c = 0; c < ACROSS; ++c) early[n][c] = sums_of(min(n, n_parts - 1), c);
+            float top = st.x;
 #pragma unroll 1
-                for (int n0 = 0; n0 < n_parts; n0 += 32) {
-                    if (n0 > 0) st = n0 + lane < n_parts ? stat_of(n0 + lane, h) : make_float2(-INFINITY, 0.f);
-                    const float mine_of = power2(st.x - from);
-                    sum += mine_of * st.y;
-                    const int n1 = min(32, n_parts - n0);
-#pragma unroll 8
-                    for (int n = 0; n < n1; ++n) {
-                        const float w = __shfl_sync(0xFFFFFFFFu, mine_of, n);
+            for (int n = lane + 32; n < n_parts; n += 32) top = fmaxf(top, stat_of(n).x);
 #pragma unroll
-                        for (int c = 0; c < (DP + 127) / 128; ++c) {
-                            const int d = 128 * c + 4 * lane;
-                            if (d < a.dim) {
-                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(n0 + n) + h * DP + d));
-                                v[c] = make_float4(v[c].x + w * x.x, v[c].y + w * x.y, v[c].z + w * x.z, v[c].w + w * x.w);
-                            }
-                        }
+            for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, i));
+            const float from = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
+            float4 v[ACROSS];
+#pragma unroll
+            for (int c = 0; c < ACROSS; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const auto add = [&](const float4 &x, float w, int c) {
+                v[c] = make_float4(v[c].x + w * x.x, v[c].y + w * x.y, v[c].z + w * x.z, v[c].w + w * x.w);
+            };
+#pragma unroll 1
+            for (int n0 = 0; n0 < n_parts; n0 += 32) {
+                if (n0 > 0) st = n0 + lane < n_parts ? stat_of(n0 + lane) : make_float2(-INFINITY, 0.f);
+                const float weight = power2(st.x - from);  // (of a part that is not there: 0)
+                sum += weight * st.y;
+                int n = 0;
+                if (n0 == 0) {
+#pragma unroll
+                    for (; n < EARLY; ++n) {
+                        const float w = __shfl_sync(0xFFFFFFFFu, weight, n);
+#pragma unroll
+                        for (int c = 0; c < ACROSS; ++c)
+                            if (n < n_parts) add(early[n][c], w, c);
                     }
                 }
+                const int n1 = min(32, n_parts - n0);
+#pragma unroll 8
+                for (; n < n1; ++n) {
+                    const float w = __shfl_sync(0xFFFFFFFFu, weight, n);
 #pragma unroll
-                for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, i);
-                const float inv = inverse_sum(sum), w = inv * a.v_scale;
-#pragma unroll
-                for (int c = 0; c < (DP + 127) / 128; ++c) {
-                    const int d = 128 * c + 4 * lane;
-                    write_output(a, f.row, head0, h * a.dim + d, make_float4(v[c].x * w, v[c].y * w, v[c].z * w, v[c].w * w), d < a.dim);
+                    for (int c = 0; c < ACROSS; ++c) add(sums_of(n0 + n, c), w, c);
                 }
-                if (WEIGHTS && lane == 0) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(top, inv * P::UP);
             }
+#pragma unroll
+            for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, i);
+            const float inv = inverse_sum(sum), w = inv * a.v_scale;
+#pragma unroll
+            for (int c = 0; c < ACROSS; ++c) {
+                const int d = 128 * c + 4 * lane;
+                write_output(a, f.row, head0, h * a.dim + d, make_float4(v[c].x * w, v[c].y * w, v[c].z * w, v[c].w * w), d < a.dim);
+            }
+            if (WEIGHTS && lane == 0) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(top, inv * P::UP);
         }
     }
 
