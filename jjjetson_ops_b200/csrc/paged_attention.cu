@@ -33,6 +33,9 @@ constexpr int BEGIN = 5;
 constexpr int STEP = 2;           // units that a warp takes at a time: two tiles of 16 rows for the tensor cores
 constexpr int SMEM_BYTES = 227 * 1024;
 
+// A product with a key is below 2^25: times this it is nothing.  (Not 0, which a key that is not seen has to be minus infinity times.)
+constexpr float LEAST_SCALE = 1e-37f;
+
 struct AttnArgs {
     const float *q;
     int64_t q_row, q_head;
@@ -565,10 +568,10 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fabsf(raw[t][s][j]));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2));
-            // 2^-e with 2^e <= largest, within 2^-100 .. 2^100
+            // 2^-e with 2^e <= largest, within 2^-126 .. 2^126
             int e = (int)(__float_as_uint(largest) >> 23) - 127;
-            e = P::N == 3 || largest == 0.f ? 0 : max(-100, min(100, e));
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23 | a.negative << 31), up = __uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2;
+            e = P::N == 3 || largest == 0.f ? 0 : max(-126, min(126, e));
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23 | a.negative << 31), up = fmaxf(__uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2, LEAST_SCALE);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) {
                 uint32_t w0[P::N], w1[P::N];
@@ -1124,7 +1127,7 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
     a.q = d_q, a.q_row = q_stride_row, a.q_head = q_stride_head;
     a.k = static_cast<const char *>(cache->d_k), a.v = static_cast<const char *>(cache->d_v);
     a.lens = d_lens, a.seqs = d_seqs, a.out = d_out, a.xq = static_cast<uint8_t *>(d_xq);
-    a.scale_log2 = std::fmax((float)(std::fabs((double)scale) * cache->k_scale * 1.4426950408889634), 1e-30f);  // (0: all logits vanish)
+    a.scale_log2 = std::fmax((float)(std::fabs((double)scale) * cache->k_scale * 1.4426950408889634), LEAST_SCALE);
     a.negative = scale < 0.f;
     a.v_scale = cache->v_scale;
     a.rows = (int)num_rows, a.q_heads = (int)num_q_heads, a.kv_heads = (int)cache->num_kv_heads, a.group = a.q_heads / a.kv_heads, a.dim = (int)dim;

@@ -64,6 +64,10 @@ __device__ __forceinline__ void store_floats(float *to, const float *from) {
     }
 }
 
+// (spelled out: every instance gives the same bits, whatever strides and alignment it was chosen for)
+__device__ __forceinline__ float turned_first(float a, float b, float c, float s) { return __fmaf_rn(a, c, -__fmul_rn(b, s)); }
+__device__ __forceinline__ float turned_second(float a, float b, float c, float s) { return __fmaf_rn(b, c, __fmul_rn(a, s)); }
+
 // One group of W pairs: where its two parts lie in a head.
 struct Unit {
     int first, second;  // offsets of the first and the second elements of the pairs (half layout) or of the halves of 2 W in a row
@@ -153,14 +157,14 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
                         const float e = y[2 * i], o = y[2 * i + 1];
-                        y[2 * i] = e * c[i] - o * s[i];
-                        y[2 * i + 1] = o * c[i] + e * s[i];
+                        y[2 * i] = turned_first(e, o, c[i], s[i]);
+                        y[2 * i + 1] = turned_second(e, o, c[i], s[i]);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
-                        y[i] = p[i] * c[i] - q[i] * s[i];
-                        y[W + i] = q[i] * c[i] + p[i] * s[i];
+                        y[i] = turned_first(p[i], q[i], c[i], s[i]);
+                        y[W + i] = turned_second(p[i], q[i], c[i], s[i]);
                     }
                 }
 #pragma unroll
