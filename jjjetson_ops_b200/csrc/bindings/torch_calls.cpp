@@ -58,6 +58,7 @@ const Binding bindings[] = {
 PyObject *bind(PyObject *, PyObject *addresses) {
     for (const Binding &b : bindings) {
         PyObject *v = PyDict_GetItemString(addresses, b.name);
+        if (v == nullptr && *b.slot != nullptr) continue;  // stays as it was bound before
         if (v == nullptr) {
             PyErr_Format(PyExc_KeyError, "no address given for %s", b.name);
             return nullptr;
@@ -573,7 +574,7 @@ PyObject *evict(PyObject *const *a, Py_ssize_t n) {
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&entry<f>)), METH_FASTCALL
 PyMethodDef methods[] = {
-    {"bind", bind, METH_O, "Addresses of the library's functions, by name."},
+    {"bind", bind, METH_O, "Addresses of the library's functions, by name; the first time of all of them."},
     {"quantize", FAST(quantize), "(x, out, order, s_mode) -> status"},
     {"mul_mat", FAST(mul_mat), "(w, xq, out, K, N, M, order, kernel) -> status"},
     {"linear", FAST(linear), "(w, x, ws, out, N, s_mode) -> status"},
