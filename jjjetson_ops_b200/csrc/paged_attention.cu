@@ -508,21 +508,29 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
         const uint32_t to = ring + slot_next * S::TILE;
         if (here.live) {
             const uint32_t own = to + my_place;
-            if (grouped && here.mask == 0xFFFFFFFFu) {
+            if (grouped) {
                 const char *from[2] = {pool + here.offset[0], pool + here.offset[1]};
+                if (here.mask == 0xFFFFFFFFu) {
 #pragma unroll
-                for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
-                    copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, from[i * AT_ONCE / UNIT], inside);
-                    from[i * AT_ONCE / UNIT] += AT_ONCE * row_stride;
+                    for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
+                        copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, from[i * AT_ONCE / UNIT], inside);
+                        from[i * AT_ONCE / UNIT] += AT_ONCE * row_stride;
+                    }
+                } else {
+                    // (a unit that is not there has a place in the pool all the same; it is not read)
+                    const uint32_t mine_of = inside ? here.mask >> (lane / S::CHUNKS) : 0;
+#pragma unroll
+                    for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
+                        const bool there = mine_of >> (i * AT_ONCE) & 1u;
+                        copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, there ? from[i * AT_ONCE / UNIT] : pool, there);
+                        from[i * AT_ONCE / UNIT] += AT_ONCE * row_stride;
+                    }
                 }
             } else {
-                // (what is not there is not read: its offset is a place in the pool all the same)
-#pragma unroll 2
+#pragma unroll 4
                 for (int i = 0; i < S::KEYS / AT_ONCE; ++i) {
                     const int r = lane / S::CHUNKS + i * AT_ONCE;
-                    const int64_t other = __shfl_sync(0xFFFFFFFFu, here.offset[0], r);  // (its chunk is that lane's)
-                    const int64_t offset = grouped ? (i * AT_ONCE < UNIT ? here.offset[0] : here.offset[1]) + (i * AT_ONCE % UNIT) * row_stride
-                                                   : other - (r % S::CHUNKS) * 16 + my_chunk * 16;
+                    const int64_t offset = __shfl_sync(0xFFFFFFFFu, here.offset[0], r) - (r % S::CHUNKS) * 16 + my_chunk * 16;  // (with that lane's chunk)
                     const bool there = inside && (here.mask >> r & 1u);
                     copy16((own ^ (spread<S::CHUNKS>(i * AT_ONCE) * 16)) + i * AT_ONCE * S::ROW, pool + (there ? offset : 0), there);
                 }
