@@ -185,9 +185,10 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const Evic
         cluster.sync();
     }
     Counts before = {__reduce_add_sync(0xFFFFFFFFu, lane < warp ? of_lane.above : 0), __reduce_add_sync(0xFFFFFFFFu, lane < warp ? of_lane.equal : 0)};
-    for (int p = 0; p < part; ++p) {
-        const Counts c = *cluster.map_shared_rank(&block_counts, p);
-        before.above += c.above, before.equal += c.equal;
+    if (part > 0) {
+        Counts c = {0, 0};
+        if (lane < part) c = *cluster.map_shared_rank(&block_counts, lane);
+        before.above += __reduce_add_sync(0xFFFFFFFFu, c.above), before.equal += __reduce_add_sync(0xFFFFFFFFu, c.equal);
     }
     for (int i = s0 + lane; i - lane < s1; i += 32) {
         bool above, equal;

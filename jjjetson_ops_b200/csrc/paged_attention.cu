@@ -932,7 +932,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 const int d = 128 * c + 4 * lane;
                 return d < a.dim ? __ldcg(reinterpret_cast<const float4 *>(part_of(i) + h * DP + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             };
-            constexpr int EARLY = 4;  // parts whose sums are on their way while the weights are made
+            constexpr int EARLY = 8;  // parts whose sums are on their way while the weights are made
             float4 early[EARLY][ACROSS];
             float2 st = lane < n_parts ? stat_of(lane) : make_float2(-INFINITY, 0.f);
 #pragma unroll
