@@ -121,8 +121,9 @@ size_t jq_paged_attention_ws_bytes(int64_t num_rows, int64_t num_q_heads, const 
  * d_weights, unless NULL: fp32 [num_rows][num_kv_heads], weights_stride floats apart; to entry i < weights_len is added what this step's
  * query heads together gave to token i.  Entries that are not seen are left as they were.  d_seqs must then be NULL.
  * d_ws: jq_paged_attention_ws_bytes() bytes, 16-byte aligned, its first JQ_PAGED_ATTENTION_COUNTERS(num_rows, num_q_heads) bytes zero
- * before the first call; every call leaves them zero again.  Calls that can overlap on the GPU (two streams, two graphs) need workspaces of their own.
- * The result does not depend on the order in which blocks run. */
+ * before the first call of these sizes; every call leaves them zero again.  Calls that can overlap on the GPU (two streams, two graphs) need workspaces of their own.
+ * The result does not depend on the order in which blocks run.  num_rows * num_kv_heads * max_pages * page_size is at most 2^33
+ * (with more than 16 query heads to a key head, or 8 of more than 128 elements, that over the passes it takes). */
 #define JQ_PAGED_ATTENTION_COUNTERS(num_rows, num_q_heads) (4u * (size_t)(num_rows) * (size_t)(num_q_heads))
 int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_stride_row, int64_t q_stride_head, int64_t num_rows,
                                    int64_t num_q_heads, const jq_kv_cache *cache, const int32_t *d_lens, const int32_t *d_seqs,

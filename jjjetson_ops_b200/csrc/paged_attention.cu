@@ -241,9 +241,8 @@ __device__ __forceinline__ Row row_at(const AttnArgs &a, const Row &own, int row
 }
 
 // Four consecutive elements of the output: element `e` of the heads of one key head's tile (their elements lie end to end), as
-// fp32 and as Q8_1.  Every lane of the warp calls it, with consecutive e; `there`: it has elements.  (Not inlined: the kernel's instructions
-// have to stay in the SM's cache.  147 KB of them, with everything inlined, made a call of one short sequence take 12.6 us, most of it
-// waiting for instructions.)
+// fp32 and as Q8_1.  Every lane of the warp calls it, with consecutive e; `there`: it has elements.  (The quantizer is some 200 instructions,
+// and called from several places.)
 __device__ __noinline__ void write_q8(uint8_t *xq, int n, int row, int n_super, int rows, int order, int s_mode, float4 v, bool there) {
     if (!there) v = make_float4(0.f, 0.f, 0.f, 0.f);
     uint32_t ds;
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     segments = __reduce_add_sync(0xFFFFFFFFu, segments);
     // Few segments: each gets blocks of its own, so that a block has one segment to put together; at most an eighth of the blocks stay
     // idle.  Many: equal stretches.
-    const bool apart = segments * 8 <= gridDim.x;
+    const bool apart = segments <= gridDim.x / 8;
     if (!apart) total += segments * BEGIN;
     uint32_t per_block = apart ? (total + gridDim.x - segments - 1) / (gridDim.x - segments) : (total + gridDim.x - 1) / gridDim.x;
     if (per_block < S::LEAST) per_block = S::LEAST;
@@ -829,7 +828,6 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
         if (i < 2 * W && (there >> i & 1u)) {
             const int i0 = 31 - __clz(starts & ((2u << i) - 1));
             const uint32_t members = members_of(i0);
-            // (loops that stay loops: instructions that are executed once come from the second-level cache, a line of eight at a time)
             const auto stat = [&](uint32_t b) { return reinterpret_cast<const float2 *>(result_of(__ffs(b) - 1) + S::HEADS * DP)[h]; };
             const float own_top = stat(1u << i).x;
             float top = -INFINITY, sum = 0.f;
@@ -1018,6 +1016,20 @@ __global__ void __launch_bounds__(256) attention_weights_kernel(const AttnArgs a
 // More than eight query heads to a key head: sixteen in one pass over the keys, where the registers hold them.
 bool takes_16_heads(int64_t group, int64_t dim) { return group > 8 && dim <= 128; }
 
+int check_heads(int64_t rows, int64_t q_heads, const jq_kv_cache *c) {
+    if (rows < 0 || q_heads <= 0) return set_error(JQ_ERR_INVALID_ARG, "attention: a size is not positive");
+    if (q_heads % c->num_kv_heads != 0)
+        return set_error(JQ_ERR_SHAPE, "attention: %lld query heads do not divide among %lld key heads", (long long)q_heads, (long long)c->num_kv_heads);
+    if (rows > 0x7FFFFFF || q_heads > 65535) return set_error(JQ_ERR_TOO_LARGE, "attention: too many rows or heads");
+    // the kernel counts units in 32 bits, with BEGIN more for every segment; and nothing that follows from these sizes overflows
+    const int64_t group = q_heads / c->num_kv_heads, heads = takes_16_heads(group, c->head_dim) ? 16 : 8;
+    const double units = (double)rows * (double)c->num_kv_heads * (double)((group + heads - 1) / heads) * (double)((c->max_pages * c->page_size + UNIT - 1) / UNIT);
+    if (units > 536870912.0)
+        return set_error(JQ_ERR_TOO_LARGE, "attention: %lld rows of %lld key heads with room for %lld tokens are more than 2^29 units of %d", (long long)rows,
+                         (long long)c->num_kv_heads, (long long)(c->max_pages * c->page_size), UNIT);
+    return JQ_OK;
+}
+
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Workspace {
@@ -1041,9 +1053,6 @@ int launch_as(cudaStream_t st, AttnArgs &a, int sm_count) {
     const auto kernel = paged_attention_kernel<T, DP, NT, WEIGHTS>;
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::SMEM, true)) return rc;
     a.tiles = (a.group + S::HEADS - 1) / S::HEADS;
-    const int64_t most = ((int64_t)a.positions + UNIT - 1) / UNIT * a.kv_heads * a.tiles * a.rows;
-    if (most > 0x7FFFFFFF)
-        return set_error(JQ_ERR_TOO_LARGE, "attention: %d rows of %d key heads with room for %d tokens are more than 2^31 units of %d", a.rows, a.kv_heads, a.positions, UNIT);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)sm_count);
     cfg.blockDim = dim3(S::THREADS);
@@ -1070,14 +1079,6 @@ int launch_type(cudaStream_t st, AttnArgs &a, int type, int sm_count) {
     if (type == JQ_KV_F16) return launch_for<KvF16, WEIGHTS>(st, a, sm_count);
     if (type == JQ_KV_BF16) return launch_for<KvBf16, WEIGHTS>(st, a, sm_count);
     return launch_for<KvE4m3, WEIGHTS>(st, a, sm_count);
-}
-
-int check_heads(int64_t rows, int64_t q_heads, const jq_kv_cache *c) {
-    if (rows < 0 || q_heads <= 0) return set_error(JQ_ERR_INVALID_ARG, "attention: a size is not positive");
-    if (q_heads % c->num_kv_heads != 0)
-        return set_error(JQ_ERR_SHAPE, "attention: %lld query heads do not divide among %lld key heads", (long long)q_heads, (long long)c->num_kv_heads);
-    if (rows > 0x7FFFFFF || q_heads > 65535) return set_error(JQ_ERR_TOO_LARGE, "attention: too many rows or heads");
-    return JQ_OK;
 }
 
 }  // namespace

@@ -296,7 +296,7 @@ int check_kv_cache(const jq_kv_cache *c, KvIndex *ix) {
     if (c->head_dim <= 0 || c->head_dim % 16 != 0 || c->head_dim > KV_MAX_DIM)
         return set_error(JQ_ERR_SHAPE, "kv cache: head_dim = %lld is not a multiple of 16 up to %lld", (long long)c->head_dim, (long long)KV_MAX_DIM);
     if (c->num_pages > 0x7FFFFFFF || c->page_size > 0x7FFFFFFF || c->num_kv_heads > 65535 || c->num_seqs > 0x7FFFFFFF ||
-        c->max_pages > 0x7FFFFFFF || (c->max_pages > 0 && c->page_size > 0x7FFFFFF0 / c->max_pages))
+        c->max_pages > 0x7FFFFFFF || (c->max_pages > 0 && c->page_size > 0x7FFFFF00 / c->max_pages))
         return set_error(JQ_ERR_TOO_LARGE, "kv cache: more than 2^31 tokens in a sequence, or pages, or sequences");
     if (c->d_k == nullptr || c->d_v == nullptr) return set_error(JQ_ERR_INVALID_ARG, "kv cache: null pointer");
     if (c->num_seqs > 0 && c->max_pages > 0 && c->d_page_table == nullptr) return set_error(JQ_ERR_INVALID_ARG, "kv cache: null page table");

@@ -223,6 +223,8 @@ def test_bad_caches_are_refused_by_every_call(native_lib, status, change):
     ("ERR_INVALID_ARG", _attend, dict(xq=64, order=2)), ("ERR_INVALID_ARG", _attend, dict(xq=64, s_mode=5)),
     ("ERR_UNSUPPORTED", _attend, dict(xq=64, descriptor=cache(head_dim=48, stride_head=48, stride_slot=96))),
     ("ERR_UNSUPPORTED", _attend, dict(xq=64, q_heads=3, descriptor=cache(num_kv_heads=1))),
+    ("ERR_TOO_LARGE", _attend, dict(rows=3, descriptor=cache(page_size=2**10, max_pages=2**21 - 1, table_stride=2**21, num_kv_heads=4, stride_page=2**18))),
+    ("ERR_TOO_LARGE", _attend, dict(rows=2**27 - 1, seqs=64, weights=None, descriptor=cache(max_pages=2**26, table_stride=2**26))),
     ("ERR_UNSUPPORTED", _attend, dict(weights=64, seqs=64)), ("ERR_INVALID_ARG", _attend, dict(weights=64, stride=3, length=4)),
     ("ERR_INVALID_ARG", _attend, dict(weights=64, length=-1)),
     ("ERR_INVALID_ARG", _attend, dict(q=None)), ("ERR_INVALID_ARG", _attend, dict(lens=None)), ("ERR_INVALID_ARG", _attend, dict(ws=None)),
@@ -240,6 +242,15 @@ def test_bad_caches_are_refused_by_every_call(native_lib, status, change):
 def test_refused_arguments(native_lib, status, call, args):
     c = native_lib
     assert call(c, c.lib(), **args) == getattr(c, status), c.last_error()
+
+
+def test_workspaces_that_would_overflow_are_refused(native_lib):
+    """Sizes whose product has more than 64 bits: an error, not a small number."""
+    lib = native_lib.lib()
+    wide = cache(num_kv_heads=65535, page_size=2**10, max_pages=2**21 - 1, table_stride=2**21, stride_page=2**40)
+    for rows in (1, 65535, 2**27 - 1):
+        assert lib.jq_paged_attention_ws_bytes(rows, 65535, ctypes.byref(wide), 1) == 0
+        assert native_lib.last_error()
 
 
 def test_plain_rope_refuses(native_lib):
