@@ -7,7 +7,7 @@
 // SM to a head.  What bounds it is latency: three histograms one after the other.
 //
 // Moving: bound by bytes, each kept row read and written once.  Into other pages all rows move at once.  Within the same pages a row may only
-// be overwritten after it was read: a block has a column of 32 bytes of all rows of a head to itself and takes the rows in their
+// be overwritten after it was read: a block has a column (32 bytes or more) of all rows of a head to itself and takes the rows in their
 // order, a tile of loads before the tile's stores (a row never moves back, so later tiles read behind all earlier stores).
 #include <cooperative_groups.h>
 
@@ -255,29 +255,32 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictArg
 }
 
 constexpr int SHIFT_THREADS = 512;
-constexpr int COLUMN = 32;  // bytes
 
-// Within the same pages: two threads have a row's 32 bytes.
+// Within the same pages: 2^shift threads have 16 bytes of a row each.
 template <typename E>
-__global__ void __launch_bounds__(SHIFT_THREADS) evict_shift_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(SHIFT_THREADS) evict_shift_kernel(const EvictArgs a, int shift) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int columns = (a.row_bytes + COLUMN - 1) / COLUMN;
+    const int wide = 16 << shift, columns = (a.row_bytes + wide - 1) / wide;
     const int head = blockIdx.y, seq = blockIdx.z;
     const bool values = (int)blockIdx.x >= columns;
     if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) write_length(a, seq);
     char *rows = values ? a.v : a.k;
-    const int chunk = ((int)blockIdx.x - (values ? columns : 0)) * COLUMN + (threadIdx.x & 1) * 16;
+    const int chunk = ((int)blockIdx.x - (values ? columns : 0)) * wide + (threadIdx.x & ((1 << shift) - 1)) * 16;
     const bool inside = chunk < a.row_bytes;
     const int64_t column = (int64_t)head * a.ix.stride_head * (int)sizeof(E) + chunk;
     const int32_t *kept = a.kept + ((int64_t)seq * a.kv_heads + head) * a.keep;
-    constexpr int ROWS = SHIFT_THREADS / 2;
-    for (int j0 = 0; j0 < a.keep && kept[j0] >= 0; j0 += ROWS * MOVE_AT_ONCE) {
+    // Indices ascend: if the last of them is in its place, all are.  (Should another block have written the new length already, in the place
+    // of the old one, this is the same number.)
+    const int stays = min(tokens_of(a, seq), a.keep);
+    if (stays == 0 || kept[stays - 1] == stays - 1) return;
+    const int rows_at_once = SHIFT_THREADS >> shift;
+    for (int j0 = 0; j0 < stays; j0 += rows_at_once * MOVE_AT_ONCE) {
         uint4 x[MOVE_AT_ONCE];
         int64_t to[MOVE_AT_ONCE];
 #pragma unroll
         for (int u = 0; u < MOVE_AT_ONCE; ++u) {
-            const int j = j0 + u * ROWS + (threadIdx.x >> 1);
+            const int j = j0 + u * rows_at_once + (int)(threadIdx.x >> shift);
             to[u] = -1;
             if (j >= a.keep || !inside) continue;
             const int i = kept[j];
@@ -318,8 +321,11 @@ int launch(cudaStream_t st, void (*kernel)(A...), dim3 grid, int threads, size_t
 template <typename E>
 int launch_move(cudaStream_t st, const EvictArgs &a, int64_t seqs, bool in_place) {
     if (in_place) {
-        const int columns = (a.row_bytes + COLUMN - 1) / COLUMN;
-        return launch(st, evict_shift_kernel<E>, dim3((unsigned)(2 * columns), (unsigned)a.kv_heads, (unsigned)seqs), SHIFT_THREADS, 0, 0, a);
+        // columns as wide as leave all rows in one tile, 32 bytes at least: 1024 rows of 256 bytes in columns of 64 11.8 us, of 32 8.2
+        int shift = 1;
+        while ((16 << shift) < a.row_bytes && ((SHIFT_THREADS * MOVE_AT_ONCE) >> (shift + 1)) >= a.keep) ++shift;
+        const int columns = (a.row_bytes + (16 << shift) - 1) / (16 << shift);
+        return launch(st, evict_shift_kernel<E>, dim3((unsigned)(2 * columns), (unsigned)a.kv_heads, (unsigned)seqs), SHIFT_THREADS, 0, 0, a, shift);
     }
     int shift = 0;
     while (16 << shift < a.row_bytes) ++shift;
@@ -377,8 +383,12 @@ int jq_kv_evict_device(void *stream, const jq_kv_cache *cache, const int32_t *d_
     a.row_bytes = (int)cache->head_dim * kv_element_bytes(cache->type);
     a.fault = device_fault_ptr();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Blocks per head: one for every 2048 weights, but no more than run at a time (two on an SM), as far as shared memory allows.
+    DeviceCaps caps;
+    if (int rc = device_caps(&caps)) return rc;
+    const int64_t heads = a.kv_heads * cache->num_seqs;
     int parts = 1;
-    while (parts < MAX_CLUSTER && max_len > 2048 * parts) parts *= 2;
+    while (parts < MAX_CLUSTER && max_len > 2048 * parts && (2 * parts * heads <= 2 * caps.sm_count || max_len > MAX_SLICE * parts)) parts *= 2;
     const size_t smem = sizeof(float) * (size_t)(((max_len + parts - 1) / parts + 31) / 32 * 32);
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(evict_select_kernel), (int)(smem > 32 * 1024 ? sizeof(float) * MAX_SLICE : 32 * 1024))) return rc;
     if (int rc = launch(st, evict_select_kernel, dim3((unsigned)(a.kv_heads * parts), (unsigned)cache->num_seqs), SELECT_THREADS, smem, parts, a)) return rc;

@@ -966,7 +966,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                     }
                 }
                 const int n1 = min(32, n_parts - n0);
-#pragma unroll 8
+#pragma unroll 16
                 for (; n < n1; ++n) {
                     const float w = __shfl_sync(0xFFFFFFFFu, weight, n);
 #pragma unroll
@@ -997,7 +997,8 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
     }
 }
 
-// Adds to every seen token's weight what its query heads gave it.  A thread a token; the logits of the attention kernel are read once.
+// Adds to every seen token's weight what its query heads gave it.  The logits of the attention kernel are read once: a thread has one token's,
+// four heads at a time where they are aligned.
 __global__ void __launch_bounds__(256) attention_weights_kernel(const AttnArgs a, float *weights, int64_t weights_stride, int64_t weights_len) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1005,11 +1006,24 @@ __global__ void __launch_bounds__(256) attention_weights_kernel(const AttnArgs a
     const Row r = row_of(a, row);
     const float2 *norms = a.norms + (int64_t)row * a.q_heads + kv_head * a.group;
     const int64_t end = min((int64_t)r.end, weights_len);
+    const int64_t segment = (int64_t)row * a.kv_heads + kv_head;
     for (int64_t key = r.first + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; key < end; key += (int64_t)gridDim.x * blockDim.x) {
-        const float *s = a.logits + (((int64_t)row * a.kv_heads + kv_head) * a.positions + key) * a.group;
+        const float *s = a.logits + (segment * a.positions + key) * a.group;
+        float *to = weights + segment * weights_stride + key;
+        const float before = *to;
         float given = 0.f;
-        for (int h = 0; h < a.group; ++h) given += power2(s[h] - norms[h].x) * norms[h].y;
-        weights[((int64_t)row * a.kv_heads + kv_head) * weights_stride + key] += given;
+        if (a.group % 4 == 0) {
+#pragma unroll 4
+            for (int h = 0; h < a.group; h += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(s + h);
+                given += power2(x.x - norms[h].x) * norms[h].y + power2(x.y - norms[h + 1].x) * norms[h + 1].y;
+                given += power2(x.z - norms[h + 2].x) * norms[h + 2].y + power2(x.w - norms[h + 3].x) * norms[h + 3].y;
+            }
+        } else {
+#pragma unroll 8
+            for (int h = 0; h < a.group; ++h) given += power2(s[h] - norms[h].x) * norms[h].y;
+        }
+        *to = before + given;
     }
 }
 
@@ -1154,8 +1168,10 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
     if (d_weights == nullptr) return launch_type<false>(st, a, cache->type, caps.sm_count);
     if (int rc = launch_type<true>(st, a, cache->type, caps.sm_count)) return rc;
     if (a.positions == 0) return JQ_OK;
-    int across = (a.positions + 255) / 256;
-    if (across > 64) across = 64;  // a block walks on where sequences are longer
+    // (blocks for eight per SM over all rows and heads at least, as far as there are tokens; they walk on where sequences are longer)
+    const int64_t segments = num_rows * a.kv_heads, most = (8 * (int64_t)caps.sm_count + segments - 1) / segments;
+    int64_t across = (a.positions + 255) / 256;
+    if (across > 16 && across > most) across = most > 16 ? most : 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)across, (unsigned)a.kv_heads, (unsigned)num_rows);
     cfg.blockDim = dim3(256);
