@@ -148,9 +148,11 @@ struct Shape {
     static constexpr int DP = DP_;                  // head_dim, padded
     static constexpr int NT = NT_;                  // tiles of eight heads
     static constexpr int HEADS = 8 * NT;
-    // A warp's accumulators and queries are its registers' larger part.  8-bit tiles are half as long on their way and need conversion: twelve
-    // warps (168 registers) where they fit, eight of them 110 us against 98 for 64 sequences of up to 5000 tokens.
-    static constexpr int WARPS = NT * DP >= 256 ? 4 : sizeof(typename T::Element) == 1 && NT == 1 && DP == 128 ? 12 : 8;
+    // A warp's accumulators and queries fill its registers.  8-bit tiles are half as long on their way and need conversion: twelve warps (168
+    // registers) where they fit, eight of them 110 us against 98 for 64 sequences of up to 5000 tokens.  Sixteen heads in one pass, or 8-bit
+    // heads of 256: eight warps with two tiles each and not four with six (20 sequences of up to 3000 tokens, 64 heads on 4, 31.8 us against
+    // 38.6; two of 93548 on e4m3, 16 heads on one, 44.6 against 69.6).  16-bit heads of 256 leave room for four.
+    static constexpr int WARPS = DP == 256 && sizeof(typename T::Element) == 2 ? 4 : sizeof(typename T::Element) == 1 && NT == 1 && DP == 128 ? 12 : 8;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROW = DP * (int)sizeof(typename T::Element);  // bytes
     static constexpr int CHUNKS = ROW / 16;
@@ -166,7 +168,7 @@ struct Shape {
     static constexpr int CHAINS = NT == 1 ? Parts<T>::N : 2;  // sums of a logit: one per part of the queries, so that they are made side by side
     static constexpr bool EARLY_QUERIES = NT * DP <= 128 && WARPS <= 8;  // the others' registers are full
     static constexpr int LEAST = WARPS * STEP;      // units of a block at least: a step for every warp
-    static_assert(SLOTS >= 3, "while one tile is read two are on their way");
+    static_assert(SLOTS >= 2, "while one tile is read another is on its way");
     static_assert(SLOTS * TILE >= RESULT + 2 * WARPS * HEADS * 12, "a warp's last result takes the place of its ring, the block's factors what is behind it");
     static_assert(2 * WARPS * HEADS <= THREADS, "a thread for every factor");
 };
@@ -966,11 +968,21 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                     }
                 }
                 const int n1 = min(32, n_parts - n0);
-#pragma unroll 16
-                for (; n < n1; ++n) {
-                    const float w = __shfl_sync(0xFFFFFFFFu, weight, n);
+                // eight parts at a time, the last ones with the weight 0
+#pragma unroll 1
+                for (; n < n1; n += 8) {
+                    float4 x[8][ACROSS];
 #pragma unroll
-                    for (int c = 0; c < ACROSS; ++c) add(sums_of(n0 + n, c), w, c);
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int c = 0; c < ACROSS; ++c) x[i][c] = sums_of(n0 + min(n + i, n1 - 1), c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float w = n + i < n1 ? __shfl_sync(0xFFFFFFFFu, weight, (n + i) & 31) : 0.f;
+#pragma unroll
+                        for (int c = 0; c < ACROSS; ++c)
+                            if (n + i < n1) add(x[i][c], w, c);
+                    }
                 }
             }
 #pragma unroll
