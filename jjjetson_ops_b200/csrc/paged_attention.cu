@@ -262,6 +262,9 @@ __device__ __forceinline__ void write_output(const AttnArgs &a, int row, int hea
     if (a.xq != nullptr) write_q8(a.xq, n, row, a.n_super, a.rows, a.order, a.s_mode, v, there);
 }
 
+// What the weights go by: a row whose pages are all bad has logits of minus infinity, which 0 and not their maximum is taken from (times 0, a
+// difference of infinities would leave NaN in the weights).
+__device__ __forceinline__ float2 norm_of(float top, float inverse) { return make_float2(top == -INFINITY ? 0.f : top, inverse); }
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }  // a row whose pages are all bad gives zeros
 
 template <typename T, int DP, int NT, bool WEIGHTS>
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                     write_output(a, row, head0, h * a.dim + d, v, d < a.dim);
                 }
             }
-            if (WEIGHTS && lane < heads) a.norms[(int64_t)row * a.q_heads + head0 + lane] = make_float2(stats[lane].x, inverse_sum(stats[lane].y) * P::UP);
+            if (WEIGHTS && lane < heads) a.norms[(int64_t)row * a.q_heads + head0 + lane] = norm_of(stats[lane].x, inverse_sum(stats[lane].y) * P::UP);
             __syncwarp();
             if (phase != MIDDLE && lane == 0) mine[phase == FIRST ? 0 : 1].n = 0;
         }
@@ -890,7 +893,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 if (whole) write_output(a, f.row, head0, h * a.dim + d, v, d < a.dim);
             }
             if (lane == 0 && !whole) __stcg(reinterpret_cast<float2 *>(part + S::HEADS * DP) + h, st);
-            if (WEIGHTS && lane == 0 && whole) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(st.x, inv * P::UP);
+            if (WEIGHTS && lane == 0 && whole) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = norm_of(st.x, inv * P::UP);
         }
         turn -= heads;
     }
@@ -993,7 +996,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 const int d = 128 * c + 4 * lane;
                 write_output(a, f.row, head0, h * a.dim + d, make_float4(v[c].x * w, v[c].y * w, v[c].z * w, v[c].w * w), d < a.dim);
             }
-            if (WEIGHTS && lane == 0) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = make_float2(top, inv * P::UP);
+            if (WEIGHTS && lane == 0) a.norms[(int64_t)f.row * a.q_heads + head0 + h] = norm_of(top, inv * P::UP);
         }
     }
 

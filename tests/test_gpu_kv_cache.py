@@ -430,6 +430,33 @@ def test_attention_bad_pages(capi):
         assert torch.equal(xq, capi.quantize_q8_1(out.view(3, 256), capi.ORDER_COL_KSUPER, capi.S_D_SUM_Q))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("tokens", [3, 40, 3000])
+def test_attention_weights_of_bad_pages(capi, kind, tokens):
+    """Tokens on pages that do not exist are given nothing: their weights stay as they were, also where a row has no other tokens (in one warp's
+    hands, a block's, or several blocks')."""
+    g = generator(41)
+    need = -(-tokens // 16)
+    k, v = pool(g, need + 1, 16, 2, 64, TYPES[kind])
+    pages = torch.arange(need, dtype=torch.int32, device="cuda").repeat(3, 1)
+    pages[1] = -1
+    pages[2, 0] = need + 1
+    q, lens = randn(g, 3, 8, 64), i32([tokens] * 3)
+    weights = torch.rand((3, 2, need * 16), generator=g, device="cuda")
+    before, out = weights.clone(), torch.empty_like(q)
+    capi.paged_attention_q8_1(q, k, v, pages, lens, out=out, want_q8=False, weights=weights)
+    assert capi.device_fault(clear=True) == capi.FAULT_BAD_PAGE
+    assert torch.equal(weights[1], before[1]) and (out[1] == 0).all()
+    assert torch.equal(weights[2, :, :16], before[2, :, :16])
+    want, shares, far, worst = attended(q, k, v, pages, [tokens] * 3, 16, 64**-0.5)
+    assert ((out.double() - want).abs() <= far).all()
+    for t in range(3):
+        for h in range(2):
+            at, share = shares[t][h]
+            expect = before[t, h][at].double() + share
+            assert ((weights[t, h][at].double() - expect).abs() <= share * worst + expect * 2 * U + 2.0**-120).all()
+
+
 def test_attention_follows_numbers_that_are_none(capi):
     """NaN among what a row sees makes its heads NaN, and no other row's."""
     g = generator(14)
