@@ -57,7 +57,9 @@ struct Counts {
     int above, equal;
 };
 
-__global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(const EvictArgs a) {
+// (two blocks on an SM, which leaves 32 registers and spills one: with one block, of 38, 128 blocks in clusters of eight take turns.  A whole
+// call, us with one / two: 17 x 4 heads of 27173 69.7 / 55.3, 2 x 8 of 20000 41.0 / 34.8, 6 x 8 of 9000 34.8 / 28.7; 8 of 100003 53.3 both)
+__global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const EvictArgs a) {
     extern __shared__ __align__(16) float w[];  // this block's slice
     __shared__ __align__(16) uint32_t bins[DIGITS][BINS];
     __shared__ uint32_t sums[SELECT_WARPS];
