@@ -65,7 +65,7 @@ void *next_trace_slot();
 
 // Device address (on the current device) of the word a kernel sets when one of its bounded waits
 // gives up; nullptr if it cannot be obtained.  Kernels receive it as a parameter.  The word keeps the highest
-// code reported: 1 a wait for a copy, 2 a wait for another rank's data, 3 a range check of the debug build.
+// code reported: 1 a wait for a copy, 2 a wait for another rank's data, 3 a range check of the debug build, 4 a page that does not exist.
 int *device_fault_ptr();
 
 // ---- range-checked debug build (-DJQ_BOUNDS_CHECK) ----------------------------------------------
