@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const E
     const int n = tokens_of(a, seq), stays = min(n, a.keep);
     const int thread = part * SELECT_THREADS + threadIdx.x, threads = parts * SELECT_THREADS;
 
-    for (int i = stays + thread; i < a.keep; i += threads) kept[i] = -1;
+    for (int64_t i = stays + thread; i < a.keep; i += threads) kept[i] = -1;  // (keep is up to 2^31 - 256: a step beyond it needs more bits)
     if (n <= a.keep) {  // all stay
         for (int i = thread; i < n; i += threads) {
             kept[i] = i;
@@ -232,17 +232,17 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const EvictArg
     const int chunk = threadIdx.x & ((1 << shift) - 1), rows = MOVE_THREADS >> shift;
     const bool inside = chunk * 16 < a.row_bytes;
     const int64_t column = (int64_t)head * a.ix.stride_head * (int)sizeof(E) + chunk * 16;
-    const int j0 = blockIdx.x * rows * MOVE_AT_ONCE + (threadIdx.x >> shift);
+    const uint32_t j0 = blockIdx.x * (uint32_t)(rows * MOVE_AT_ONCE) + (threadIdx.x >> shift);  // (the last block's may be above 2^31)
     uint4 k[MOVE_AT_ONCE], v[MOVE_AT_ONCE];
     int64_t to[MOVE_AT_ONCE];
 #pragma unroll
     for (int u = 0; u < MOVE_AT_ONCE; ++u) {
-        const int j = j0 + u * rows;
+        const uint32_t j = j0 + u * rows;
         to[u] = -1;
-        if (j >= a.keep || !inside) continue;
+        if (j >= (uint32_t)a.keep || !inside) continue;
         const int i = kept[j];
         if (i < 0) continue;
-        const int64_t from = place_of(a.ix, seq, i, a.fault), there = place_of(a.to, seq, j, a.fault);
+        const int64_t from = place_of(a.ix, seq, i, a.fault), there = place_of(a.to, seq, (int)j, a.fault);
         if (from < 0 || there < 0) continue;
         to[u] = there * (int)sizeof(E) + column;
         k[u] = __ldcs(reinterpret_cast<const uint4 *>(a.k + from * (int)sizeof(E) + column));
@@ -331,7 +331,7 @@ int launch_move(cudaStream_t st, const EvictArgs &a, int64_t seqs, bool in_place
     }
     int shift = 0;
     while (16 << shift < a.row_bytes) ++shift;
-    const int rows = (MOVE_THREADS >> shift) * MOVE_AT_ONCE;
+    const int64_t rows = (MOVE_THREADS >> shift) * MOVE_AT_ONCE;
     return launch(st, evict_move_kernel<E>, dim3((unsigned)((a.keep + rows - 1) / rows), (unsigned)a.kv_heads, (unsigned)seqs), MOVE_THREADS, 0, 0, a, shift);
 }
 

@@ -696,6 +696,32 @@ def test_evict_bad_pages_and_refusals(capi):
         capi.kv_evict(w, i32([12, 3]), k, v, i32([[0, 1, 2]]), 4)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_budget_next_to_2_31(capi, in_place):
+    """The largest budget that is taken: indices one step beyond it have more than 31 bits, and nothing outside the list is written."""
+    keep, edge, S = 0x7FFFFF00, 1 << 14, 40
+    g = generator(27)
+    k, v = pool(g, 7, 16, 1, 16, torch.float16)
+    k0, v0 = k.clone(), v.clone()
+    pages = i32([[5, 0, 3]])
+    new_pages = None
+    if not in_place:
+        new_pages = torch.full((1, keep // 16), -1, dtype=torch.int32, device="cuda")
+        new_pages[0, :3] = i32([6, 2, 1])
+    around = torch.full((keep + 2 * edge,), 7, dtype=torch.int32, device="cuda")
+    kept = around[edge:edge + keep].view(1, 1, keep)
+    w = torch.rand((1, 1, S), generator=g, device="cuda")
+    w0 = w.clone()
+    _, n = capi.kv_evict(w, i32([S]), k, v, pages, keep, new_page_table=new_pages, kept=kept)
+    assert n.item() == S and torch.equal(w, w0)
+    assert (around[:edge] == 7).all() and (around[edge + keep:] == 7).all()
+    assert kept[0, 0, :S].tolist() == list(range(S)) and kept[0, 0, S:].amax().item() == -1 and kept[0, 0, S:].amin().item() == -1
+    if not in_place:
+        for old, new, slots in ((5, 6, 16), (0, 2, 16), (3, 1, 8)):
+            k0[new, :slots], v0[new, :slots] = k0[old, :slots], v0[old, :slots]
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
 # ---- all of it, the way a decoder uses it --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("graph", [False, True])
