@@ -121,7 +121,10 @@ size_t jq_paged_attention_ws_bytes(int64_t num_rows, int64_t num_q_heads, const 
  * d_weights, unless NULL: fp32 [num_rows][num_kv_heads], weights_stride floats apart; to entry i < weights_len is added what this step's
  * query heads together gave to token i.  Entries that are not seen are left as they were.  d_seqs must then be NULL.
  * d_ws: jq_paged_attention_ws_bytes() bytes, 16-byte aligned, its first JQ_PAGED_ATTENTION_COUNTERS(num_rows, num_q_heads) bytes zero
- * before the first call of these sizes; every call leaves them zero again.  Calls that can overlap on the GPU (two streams, two graphs) need workspaces of their own.
+ * before the first call.  One workspace serves calls of any sizes, caches and types one after the other, as long as it has the bytes of
+ * each, and that many bytes of the call with the most rows and heads (4096 are enough for all) were zero before the first of them: what
+ * counts lies in the same place in all, and every call leaves it zero again.  Calls that can overlap on the GPU (two streams, two graphs)
+ * need workspaces of their own.
  * The result does not depend on the order in which blocks run.  num_rows * num_kv_heads * max_pages * page_size is at most 2^33
  * (with more than 16 query heads to a key head, or 8 of more than 128 elements, that over the passes it takes). */
 #define JQ_PAGED_ATTENTION_COUNTERS(num_rows, num_q_heads) (4u * (size_t)(num_rows) * (size_t)(num_q_heads))

@@ -314,13 +314,13 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
 
 def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor, weights: bool = False) -> torch.Tensor:
     """Workspace of ``paged_attention_q8_1`` for queries, caches and tables of these shapes, whatever the lengths; ``weights``: for
-    calls that accumulate weights.  It serves call after call of these sizes on one stream; calls that can overlap, and calls of other
-    numbers of rows or heads, need one each."""
+    calls that accumulate weights.  It serves call after call on one stream, of these sizes and of any others that need no more bytes
+    (no more rows, heads and pages); calls that can overlap need one each."""
     n = _calls.attention_ws_bytes(q, k_cache, page_table, weights)
     if n == 0:
         raise JqError(ERR_INVALID_ARG, last_error())
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    ws[: 4 * q.shape[0] * q.shape[1]].zero_()  # the counters
+    ws[:4096].zero_()  # the counters, of calls of any size
     return ws
 
 

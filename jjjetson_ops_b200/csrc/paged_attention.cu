@@ -51,7 +51,7 @@ struct AttnArgs {
     int tiles;         // parts of a group that are computed apart (groups of more heads than one pass takes)
     int n_super, order, s_mode;
     // workspace
-    int *counters;
+    int *counters;     // one for every segment that blocks share: never more than there are blocks
     float *parts;
     float2 *norms;     // [rows][q_heads]: largest logit, 1 / sum (with weights)
     float *logits;     // [rows][kv_heads][positions][group] (with weights)
@@ -910,7 +910,9 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 n_parts = (start + f.units - 1) / per_block - first + 1;
             }
             part_first[threadIdx.x] = first, part_count[threadIdx.x] = n_parts;
-            int *counter = a.counters + (int64_t)f.row * segments_row + f.segment;
+            // Where segments are many they go by the block that they begin in: of those that go on behind it a block has one.  So the counters
+            // are as many as blocks at most, and lie in the same place for calls of any size.
+            int *counter = a.counters + ((int64_t)a.rows * segments_row <= gridDim.x ? f.row * segments_row + f.segment : first);
             asm volatile("fence.acq_rel.gpu;\n\tatom.acq_rel.gpu.global.add.s32 %0, [%1], 1;\n\tfence.acq_rel.gpu;" : "=r"(before) : "l"(counter) : "memory");
             if (before == n_parts - 1) *counter = 0;  // for the next call
             is_last[threadIdx.x] = before == n_parts - 1;
@@ -1067,12 +1069,13 @@ struct Workspace {
 int workspace_of(int64_t rows, int64_t q_heads, const jq_kv_cache *c, bool weights, Workspace *w) {
     DeviceCaps caps;
     if (int rc = device_caps(&caps)) return rc;
-    w->parts = rounded(JQ_PAGED_ATTENTION_COUNTERS(rows, q_heads));
+    w->parts = rounded(sizeof(int) * (size_t)caps.sm_count);  // behind the counters, of which there is one for a block at most
     const int64_t dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256, heads = takes_16_heads(q_heads / c->num_kv_heads, c->head_dim) ? 16 : 8;
     const size_t part = heads * dim + 2 * heads;  // floats: Shape::PART of the instance that launch_for() takes
     w->norms = w->parts + rounded(2 * (size_t)caps.sm_count * part * sizeof(float));
     w->logits = w->norms + (weights ? rounded(sizeof(float2) * (size_t)rows * q_heads) : 0);
     w->total = w->logits + (weights ? rounded(sizeof(float) * (size_t)rows * q_heads * (size_t)(c->max_pages * c->page_size)) : 0);
+    if (w->total < JQ_PAGED_ATTENTION_COUNTERS(rows, q_heads)) w->total = rounded(JQ_PAGED_ATTENTION_COUNTERS(rows, q_heads));  // (which the caller zeroes)
     return JQ_OK;
 }
 

@@ -506,6 +506,27 @@ def test_attention_workspace(capi):
         capi.paged_attention_q8_1(q, k, v, pages, i32(lens), weights=w, ws=capi.paged_attention_workspace(q, k, pages))
 
 
+@pytest.mark.parametrize("made_for", [64, 1])
+def test_attention_workspace_of_changing_batches(capi, made_for):
+    """A batch that grows and shrinks, and caches of other heads and types, in one workspace: the bits of a workspace of its own each time."""
+    g = generator(42)
+    calls = []
+    for kind, Hq, Hk, D, lens in (("f16", 32, 8, 128, [900] * 64), ("f16", 32, 8, 128, [6000]), ("f16", 32, 8, 128, [3000, 0, 17]),
+                                  ("e4m3", 4, 1, 64, [5000, 700]), ("bf16", 16, 2, 128, [40] * 150), ("f16", 32, 8, 128, [1, 900] * 32)):
+        pages, total = table_for(g, lens, 16)
+        k, v = pool(g, total, 16, Hk, D, TYPES[kind])
+        calls.append((randn(g, len(lens), Hq, D), k, v, pages, i32(lens)))
+    alone = [torch.full_like(c[0], 9.0) for c in calls]
+    for call, out in zip(calls, alone):
+        capi.paged_attention_q8_1(*call, out=out, want_q8=False)
+    q, k, v, pages, lens = calls[0]
+    ws = capi.paged_attention_workspace(q[:made_for], k, pages[:made_for])
+    for i in (0, 1, 0, 2, 3, 0, 4, 1, 5, 3, 4, 0):
+        out = torch.full_like(alone[i], 9.0)
+        capi.paged_attention_q8_1(*calls[i], out=out, want_q8=False, ws=ws)
+        assert torch.equal(out, alone[i]), i
+
+
 def test_attention_in_graphs_and_on_other_streams(capi):
     """Two graphs with workspaces of their own, replayed at once with lengths that change in between; an eager call on a third stream."""
     g = generator(17)
