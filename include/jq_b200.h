@@ -303,10 +303,11 @@ int jq_quantize_q4_0_device(void *stream, const float *d_w, void *d_wq, int64_t 
 
 /* *fault_out is non-zero after a kernel of this library gave up on a bounded wait on the current device
  * (1: a bulk copy or pipeline stage never completed; 2: the bands of an all-gather never arrived), or, in the
- * range-checked debug build, skipped an access that fell outside its buffer (3); the word keeps the highest
+ * range-checked debug build, skipped an access that fell outside its buffer (3); of several the highest
  * code.  The call then returns JQ_ERR_TIMEOUT, else JQ_OK.  (4, with JQ_ERR_INVALID_ARG: a page table named a page
- * that its cache does not have; see jq_kv_cache.h.)  The kernel has returned, its output is not
- * valid, and the device stays usable.  Synchronises the device.  `clear` != 0 resets the word. */
+ * that its cache does not have; see jq_kv_cache.h.  1 to 3 are reported before it.)  The kernel has returned, its output is not
+ * valid, and the device stays usable.  Synchronises the device.  `clear` != 0 forgets what was reported: 1 to 3
+ * together, or 4, so that a 4 beside them is what the next call reports. */
 int jq_device_fault(int clear, int *fault_out);
 
 /* The range-checked debug build (compiled with -DJQ_BOUNDS_CHECK, linked as libjq_b200_check.so) stands in

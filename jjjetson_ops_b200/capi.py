@@ -485,9 +485,9 @@ def quantize_q4_0(w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.
 
 
 def device_fault(clear: bool = True) -> int:
-    """The device's fault word (0: no bounded wait has given up, no page table named a page that does not exist).  A
-    non-zero word comes with status JQ_ERR_TIMEOUT (``FAULT_BAD_PAGE``: JQ_ERR_INVALID_ARG), which is reported through
-    the return value here, not raised."""
+    """The device's fault code (0: no bounded wait has given up, no page table named a page that does not exist).  A
+    code comes with status JQ_ERR_TIMEOUT (``FAULT_BAD_PAGE``, which is reported after the others: JQ_ERR_INVALID_ARG), which
+    is reported through the return value here, not raised.  ``clear`` forgets what was reported."""
     v = ctypes.c_int(0)
     rc = _lib.jq_device_fault(1 if clear else 0, ctypes.byref(v))
     if rc not in (OK, ERR_TIMEOUT) and not (rc == ERR_INVALID_ARG and v.value == FAULT_BAD_PAGE):

@@ -22,7 +22,7 @@ namespace {
 
 thread_local std::string t_last_error;
 
-__device__ int g_device_fault_word = 0;
+__device__ int g_device_fault_words[FAULT_CODES] = {};
 
 constexpr int MAX_DEVICES = 64;
 struct PerDevice {
@@ -157,7 +157,7 @@ int *device_fault_ptr() {
     PerDevice &d = g_dev[dev];
     if (!d.fault_ok) {
         void *p = nullptr;
-        if (cudaGetSymbolAddress(&p, g_device_fault_word) != cudaSuccess) {
+        if (cudaGetSymbolAddress(&p, g_device_fault_words) != cudaSuccess) {
             (void)cudaGetLastError();
             return nullptr;
         }
@@ -762,16 +762,24 @@ int jq_quantize_q4_0_device(void *stream, const float *d_w, void *d_wq, int64_t 
 
 int jq_device_fault(int clear, int *fault_out) {
     int *p = device_fault_ptr();
-    if (p == nullptr) return set_error(JQ_ERR_CUDA, "cannot locate the device fault word");
-    int v = 0;
+    if (p == nullptr) return set_error(JQ_ERR_CUDA, "cannot locate the device fault words");
+    int words[FAULT_CODES] = {};
     JQ_CUDA_TRY(cudaDeviceSynchronize());
-    JQ_CUDA_TRY(cudaMemcpy(&v, p, sizeof(int), cudaMemcpyDeviceToHost));
+    JQ_CUDA_TRY(cudaMemcpy(words, p, sizeof(words), cudaMemcpyDeviceToHost));
+    // Results that are not valid go first; a page that does not exist is reported when they have been.
+    constexpr int PAGE = FAULT_CODES - 1;
+    int v = 0;
+    for (int i = 0; i < PAGE; ++i) {
+        if (words[i] != 0) v = i + 1;
+    }
+    const bool page = v == 0 && words[PAGE] != 0;
+    if (page) v = FAULT_CODES;
     if (clear && v != 0) {
-        const int zero = 0;
-        JQ_CUDA_TRY(cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice));
+        const int zeros[FAULT_CODES] = {};
+        JQ_CUDA_TRY(cudaMemcpy(page ? p + PAGE : p, zeros, sizeof(int) * (page ? 1 : PAGE), cudaMemcpyHostToDevice));
     }
     if (fault_out) *fault_out = v;
-    if (v == 4)
+    if (page)
         return set_error(JQ_ERR_INVALID_ARG, "a page table named a page that the cache does not have: its tokens were neither written nor attended to");
     if (v == 3)
         return set_error(JQ_ERR_TIMEOUT, "a range check of the debug build failed: an access outside its buffer was skipped");

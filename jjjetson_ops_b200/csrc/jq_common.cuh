@@ -63,9 +63,10 @@ uint32_t copy_wait_poll_limit();
 // per-CTA timestamps, or nullptr when tracing is off or the buffer is full.
 void *next_trace_slot();
 
-// Device address (on the current device) of the word a kernel sets when one of its bounded waits
-// gives up; nullptr if it cannot be obtained.  Kernels receive it as a parameter.  The word keeps the highest
-// code reported: 1 a wait for a copy, 2 a wait for another rank's data, 3 a range check of the debug build, 4 a page that does not exist.
+// Device address (on the current device) of the words a kernel sets when one of its bounded waits
+// gives up; nullptr if it cannot be obtained.  Kernels receive it as a parameter.  Every code has a word of its own,
+// so that none hides another: 1 a wait for a copy, 2 a wait for another rank's data, 3 a range check of the debug build, 4 a page that does not exist.
+constexpr int FAULT_CODES = 4;
 int *device_fault_ptr();
 
 // ---- range-checked debug build (-DJQ_BOUNDS_CHECK) ----------------------------------------------
@@ -236,13 +237,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// The fault word keeps the highest code reported (see device_fault_ptr()).
+// The code's own word (see device_fault_ptr()); `code` is a constant of the call.
 __device__ __forceinline__ void report_fault(int *fault, int code) {
-#ifdef JQ_BOUNDS_CHECK
-    if (fault != nullptr) atomicMax(fault, code);
-#else
-    if (fault != nullptr) atomicExch(fault, code);
-#endif
+    if (fault != nullptr) atomicExch(fault + (code - 1), code);
 }
 
 // Range checks of the debug build: true when [p, p + n) lies inside the extent (always, in a normal build).

@@ -21,7 +21,7 @@ inline int kv_element_bytes(int type) { return type == JQ_KV_E4M3 ? 1 : 2; }
 #ifdef __CUDACC__
 
 __device__ __forceinline__ void report_bad_page(int *fault) {
-    if (fault != nullptr) atomicMax(fault, FAULT_BAD_PAGE);
+    report_fault(fault, FAULT_BAD_PAGE);
 }
 
 struct KvF16 {

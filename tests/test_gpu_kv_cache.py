@@ -226,6 +226,36 @@ def test_rope_append_padding_and_bad_pages(capi):
     assert torch.equal(v[0, 15], qkv.view(7, 8, 64)[0, 6:].half())
 
 
+@pytest.mark.parametrize("page_first", [False, True])
+def test_a_bad_page_hides_no_wait_that_gave_up(capi, page_first):
+    """Whichever came first: the wait, whose results are not valid, is reported, then the page; neither is lost when the other is cleared."""
+    table, _ = capi.rope_table(16, device="cuda")
+    k, v = pool(generator(2), 1, 1, 1, 16, torch.float16)
+    flags, epoch = torch.zeros(64, dtype=torch.int32, device="cuda"), i32([1])
+
+    def bad_page():
+        capi.rope_append(torch.zeros((1, 32), device="cuda"), i32([0]), table, k, v, i32([[1]]), i32([0]))
+        torch.cuda.synchronize()
+
+    def wait_for_nothing():  # bands that no rank sends: 4096 looks, then the kernel returns
+        capi.set_option(capi.OPT_WAIT_POLL_LIMIT, 4096)
+        try:
+            capi.allgather_wait(flags.device, flags.data_ptr(), 1, epoch)
+            torch.cuda.synchronize()
+        finally:
+            capi.set_option(capi.OPT_WAIT_POLL_LIMIT, 0)
+
+    for report in (bad_page, wait_for_nothing) if page_first else (wait_for_nothing, bad_page):
+        report()
+    code = capi.ctypes.c_int(0)
+    read = lambda clear: (capi.lib().jq_device_fault(clear, capi.ctypes.byref(code)), code.value)  # noqa: E731
+    assert read(0) == (capi.ERR_TIMEOUT, 2)
+    assert read(1) == (capi.ERR_TIMEOUT, 2)
+    assert read(0) == (capi.ERR_INVALID_ARG, capi.FAULT_BAD_PAGE)
+    assert read(1) == (capi.ERR_INVALID_ARG, capi.FAULT_BAD_PAGE)
+    assert read(1) == (capi.OK, 0)
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_rope_append_values_beyond_the_type(capi, kind):
     table, _ = capi.rope_table(16, device="cuda")
