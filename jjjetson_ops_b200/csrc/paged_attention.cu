@@ -1138,6 +1138,7 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
     if (int rc = check_heads(num_rows, num_q_heads, cache)) return rc;
     if (window < 0) return set_error(JQ_ERR_INVALID_ARG, "attention: negative window");
     if (!std::isfinite(scale)) return set_error(JQ_ERR_INVALID_ARG, "attention: scale is not finite");
+    if (num_rows == 0) return JQ_OK;  // (before the outputs: an empty tensor has no address)
     if (d_out == nullptr && d_xq == nullptr) return set_error(JQ_ERR_INVALID_ARG, "attention: no output requested");
     const int64_t dim = cache->head_dim;
     if (d_xq != nullptr) {
@@ -1153,7 +1154,6 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
         if (num_rows > 65535) return set_error(JQ_ERR_TOO_LARGE, "attention: more than 65535 rows with weights");
         if (weights_len < 0 || weights_stride < weights_len) return set_error(JQ_ERR_INVALID_ARG, "attention: rows of the weights overlap");
     }
-    if (num_rows == 0) return JQ_OK;
     if (d_q == nullptr || d_lens == nullptr || d_ws == nullptr) return set_error(JQ_ERR_INVALID_ARG, "attention: null pointer");
     const uintptr_t bits = (uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_xq | (uintptr_t)d_ws | (uintptr_t)(4 * q_stride_row) | (uintptr_t)(4 * q_stride_head);
     if ((bits & 15u) != 0) return set_error(JQ_ERR_ALIGN, "attention: queries, outputs and workspace must be 16-byte aligned");

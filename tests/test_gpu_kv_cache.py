@@ -594,6 +594,16 @@ def test_attention_in_graphs_and_on_other_streams(capi):
         assert torch.equal(eager, outs[0])
 
 
+@pytest.mark.parametrize("want_q8", [False, True])
+def test_attention_without_rows(capi, want_q8):
+    """As the other calls: a batch that has become empty is no error, whichever outputs are asked for."""
+    k, v = pool(generator(20), 2, 16, 2, 64, torch.float16)
+    q, out = torch.empty((0, 4, 64), device="cuda"), torch.empty((0, 4, 64), device="cuda")
+    for table in (i32([[0, 1]]), torch.empty((0, 2), dtype=torch.int32, device="cuda")):
+        capi.paged_attention_q8_1(q, k, v, table, i32([]), out=out, want_q8=want_q8)
+        capi.paged_attention_q8_1(q, k, v, table, i32([]), out=out, want_q8=want_q8, weights=torch.empty((0, 2, 32), device="cuda"))
+
+
 def test_attention_from_strided_queries(capi):
     g = generator(18)
     k, v = pool(g, 4, 16, 2, 64, torch.float16)

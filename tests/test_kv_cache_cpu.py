@@ -244,6 +244,16 @@ def test_refused_arguments(native_lib, status, call, args):
     assert call(c, c.lib(), **args) == getattr(c, status), c.last_error()
 
 
+def test_calls_without_rows_need_no_buffers(native_lib):
+    """Empty tensors have no address: which of them there are does not matter."""
+    c, lib = native_lib, native_lib.lib()
+    assert _attend(c, lib, rows=0, out=None) == c.OK
+    assert _attend(c, lib, rows=0, out=None, q=None, lens=None, ws=None) == c.OK
+    assert _attend(c, lib, rows=0, out=None, xq=64) == c.OK
+    assert _append(c, lib, rows=0, qkv=None, q=None, positions=None, idx=None) == c.OK
+    assert _attend(c, lib, rows=0, window=-1) == c.ERR_INVALID_ARG
+
+
 def test_workspaces_that_would_overflow_are_refused(native_lib):
     """Sizes whose product has more than 64 bits: an error, not a small number."""
     lib = native_lib.lib()
