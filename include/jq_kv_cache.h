@@ -84,8 +84,8 @@ int jq_rope_table_from(const double *radians, int64_t n_pairs, uint64_t *table_o
 /* Rotates the first rotary_dim elements (even, at most head_dim) of every head of every row by the row's position and copies the
  * others: x = d_x[row * x_stride_row + head * x_stride_head ...], out likewise.  A pair (a, b) becomes
  * (a cos - b sin, b cos + a sin) * mscale.  Pairs are elements i and i + rotary_dim / 2 (interleaved = 0) or 2i and 2i + 1
- * (interleaved = 1).  d_out may be d_x with the same strides, else the two must not overlap.  head_dim is even.  The reference's
- * rope_neox is interleaved = 0 with the whole head (src/cuda/rope_neox.cu:14). */
+ * (interleaved = 1).  d_out may be d_x with the same strides, else the two must not overlap.  head_dim is even, at most 1024; rows and
+ * heads may begin at any float (with 16-byte aligned ones it is faster).  The reference's rope_neox is interleaved = 0 with the whole head (src/cuda/rope_neox.cu:14). */
 int jq_rope_device(void *stream, const float *d_x, float *d_out, const int32_t *d_positions, const uint64_t *d_table,
                    int64_t num_rows, int64_t num_heads, int64_t head_dim, int64_t rotary_dim, int64_t x_stride_row,
                    int64_t x_stride_head, int64_t out_stride_row, int64_t out_stride_head, int interleaved, float mscale);

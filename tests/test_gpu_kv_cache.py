@@ -144,6 +144,27 @@ def test_rope_strides_and_alignment(capi):
     assert torch.equal(capi.rope(row, positions, table), capi.rope(row.contiguous(), positions, table))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,D,R,shift", [(3, 2, 1024, 1024, 1), (2, 3, 1024, 1022, 0), (2, 1, 1022, 1022, 3), (5, 2, 1022, 6, 2), (3, 2, 514, 514, 1),
+                                           (700, 3, 514, 258, 0), (1, 2, 1022, 1020, 2), (2, 2, 516, 512, 1)])
+def test_rope_wide_heads_of_any_alignment(capi, T, H, D, R, shift, interleaved):
+    """Heads with more pairs than a block has threads: taken pair by pair where they begin at any float, or do not divide by four."""
+    g = generator(D + R + shift)
+    wide = randn(g, T, H, D + 5)
+    x = wide[..., shift:shift + D]
+    positions = torch.randint(0, 100000, (T,), generator=g, device="cuda", dtype=torch.int32)
+    table, mscale = capi.rope_table(R, 10000.0, device="cuda")
+    want, size = rotated(x, positions, [10000.0 ** (-2.0 * i / R) for i in range(R // 2)], 1.0, interleaved)
+    got = capi.rope(x, positions, table, interleaved=interleaved, mscale=mscale)
+    assert ((got.double() - want).abs() <= rope_bound(size, positions)).all()
+    assert torch.equal(got[..., R:], x[..., R:])
+    before = wide.clone()
+    capi.rope(x, positions, table, interleaved=interleaved, mscale=mscale, out=x)  # where it lies
+    assert torch.equal(x, got)
+    before[..., shift:shift + D] = got
+    assert torch.equal(wide, before)
+
+
 def test_rope_refuses_what_does_not_fit(capi):
     table, _ = capi.rope_table(64, device="cuda")
     x = torch.zeros((2, 3, 32), device="cuda")
