@@ -33,9 +33,6 @@ constexpr int BEGIN = 5;
 constexpr int STEP = 2;           // units that a warp takes at a time: two tiles of 16 rows for the tensor cores
 constexpr int SMEM_BYTES = 227 * 1024;
 
-// A product with a key is below 2^25: times this it is nothing.  (Not 0, which a key that is not seen has to be minus infinity times.)
-constexpr float LEAST_SCALE = 1e-37f;
-
 struct AttnArgs {
     const float *q;
     int64_t q_row, q_head;
@@ -44,8 +41,8 @@ struct AttnArgs {
     const int32_t *lens, *seqs;
     float *out;
     uint8_t *xq;
-    float scale_log2;   // |scale| * k_scale / ln 2, not zero
-    uint32_t negative;  // scale is
+    float scale;       // times 2^scale_exponent: scale * k_scale / ln 2.  Zero, or its size is in [1, 2]
+    int scale_exponent;
     float v_scale;
     int rows, q_heads, kv_heads, group, dim, window;
     int tiles;         // parts of a group that are computed apart (groups of more heads than one pass takes)
@@ -98,6 +95,7 @@ template <>
 struct Parts<KvF16> {
     static constexpr int N = 2;
     static constexpr float UP = 16384.f;  // probabilities are held times 2^14: of a million keys as small as 2^-36 nothing is lost
+    static constexpr int ROOM = 0, MOST = 100;  // see the queries: a product is below 4 * 2^16 * 256 = 2^26
     static __device__ __forceinline__ void split(float a, float b, uint32_t (&w)[N]) {
         const __half2 h = __floats2half2_rn(a, b);
         const float2 f = __half22float2(h);
@@ -113,6 +111,7 @@ template <>
 struct Parts<KvBf16> {
     static constexpr int N = 3;
     static constexpr float UP = 1.f;
+    static constexpr int ROOM = 16, MOST = 127;  // with keys up to 2^128 a product is below 2^-14 * 2^128 * 256 = 2^122
     static __device__ __forceinline__ void split(float a, float b, uint32_t (&w)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -569,7 +568,9 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
         float unscale[NT][2];
         float o[NT][DP / 16][4];
         float m[NT][2], l[NT][2];
-        // queries: two or three operands per 16 elements, scaled by a power of two so that fp16 holds them
+        // Queries: two or three operands per 16 elements, times the scale and a power of two so that fp16, or a product with bf16's largest keys,
+        // holds them.  What is left of the scale, `unscale`, is a power of two: logits are exact multiples of the products, so that however large
+        // they are the largest one's difference from itself is nothing (a rounded factor would leave it off by half a bit of the logit).
         if (!S::EARLY_QUERIES) ask_queries();
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -580,10 +581,13 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
                 for (int j = 0; j < 4; ++j) largest = fmaxf(largest, fabsf(raw[t][s][j]));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2));
-            // 2^-e with 2^e <= largest, within 2^-126 .. 2^126
-            int e = (int)(__float_as_uint(largest) >> 23) - 127;
-            e = P::N == 3 || largest == 0.f ? 0 : max(-126, min(126, e));
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23 | a.negative << 31), up = fmaxf(__uint_as_float((uint32_t)(127 + e) << 23) * a.scale_log2, LEAST_SCALE);
+            // 2^-e with 2^e <= largest (times 2^ROOM), within 2^-126 .. 2^126
+            int e = (int)(__float_as_uint(largest) >> 23) - 127 + P::ROOM;
+            e = largest == 0.f ? 0 : max(-126, min(126, e));
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23) * a.scale;
+            // not 0, which a key that is not seen has to be minus infinity times; and no finite product becomes an infinite logit, but with bf16
+            e = max(-149, min(P::MOST, e + a.scale_exponent));
+            const float up = __uint_as_float(e >= -126 ? (uint32_t)(127 + e) << 23 : 1u << (149 + e));
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s) {
                 uint32_t w0[P::N], w1[P::N];
@@ -651,7 +655,7 @@ __global__ void __launch_bounds__(Shape<T, DP, NT>::THREADS, 1) paged_attention_
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                // x: products of the scaled queries; logits in base 2 are x times unscale (which is positive)
+                // x: products of the scaled queries; logits in base 2 are x times unscale (a power of two)
                 float x[2][4];
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
@@ -1168,8 +1172,8 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
     a.q = d_q, a.q_row = q_stride_row, a.q_head = q_stride_head;
     a.k = static_cast<const char *>(cache->d_k), a.v = static_cast<const char *>(cache->d_v);
     a.lens = d_lens, a.seqs = d_seqs, a.out = d_out, a.xq = static_cast<uint8_t *>(d_xq);
-    a.scale_log2 = std::fmax((float)(std::fabs((double)scale) * cache->k_scale * 1.4426950408889634), LEAST_SCALE);
-    a.negative = scale < 0.f;
+    a.scale = 2.f * (float)std::frexp((double)scale * cache->k_scale * 1.4426950408889634, &a.scale_exponent);
+    a.scale_exponent -= 1;
     a.v_scale = cache->v_scale;
     a.rows = (int)num_rows, a.q_heads = (int)num_q_heads, a.kv_heads = (int)cache->num_kv_heads, a.group = a.q_heads / a.kv_heads, a.dim = (int)dim;
     a.positions = (int)(cache->max_pages * cache->page_size);

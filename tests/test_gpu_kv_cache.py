@@ -445,6 +445,55 @@ def test_attention_scales(capi, kind, scale, q_size, negative):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e8, 1e9, 1e12, 1e20, 1e30])
+@pytest.mark.parametrize("tokens", [20, 300, 5000])
+def test_attention_logits_of_any_size(capi, kind, size, tokens):
+    """One key that is far ahead of the others: it is given all, however large its logit (a bit of which may be a thousand)."""
+    g = generator(43)
+    Hk, G, D, need = 2, 3, 64, -(-tokens // 16)
+    k, v = pool(g, need, 16, Hk, D, TYPES[kind])
+    k.copy_((torch.rand(k.shape, generator=g, device="cuda") / 4).to(TYPES[kind]))
+    q = randn(g, 2, Hk * G, D)
+    q += q.sign() * 0.5
+    at = [3, 17, tokens - 1]
+    pages = torch.arange(need, dtype=torch.int32, device="cuda").repeat(2, 1)
+    # q . sign(q) * 2 = 2 |q|: 160 or so; of another head 2 q . sign(q'): 40 at most; of the rest |q| / 4
+    q[1] = q[0]
+    for h in range(Hk):
+        for i in range(G):
+            k[at[i] // 16, at[i] % 16, h] = (2 * q[0, h * G + i].sign()).to(TYPES[kind])
+    q *= size
+    weights, out = torch.zeros((2, Hk, need * 16), device="cuda"), torch.empty_like(q)
+    scale = D**-0.5
+    for w in (None, weights):
+        capi.paged_attention_q8_1(q, k, v, pages, i32([tokens, tokens]), scale=scale, k_scale=0.125, v_scale=0.25, out=out, want_q8=False, weights=w)
+        for h in range(Hk):
+            for i in range(G):
+                want = v[at[i] // 16, at[i] % 16, h].double() * 0.25
+                # p = 1 in parts of 22 bits, 4 u; a step's products 2 u; sums over steps, warps and blocks with zeros; 1 / l, its factor and the product
+                assert ((out[:, h * G + i].double() - want).abs() <= 20 * U * want.abs()).all(), (h, i)
+    gained = torch.zeros_like(weights).double()
+    for i in range(G):
+        gained[:, :, at[i]] += 1
+    assert ((weights.double() - gained).abs() <= 20 * U * gained).all()
+
+
+@pytest.mark.parametrize("key,scale", [(1e38, 0.0), (1e30, 0.0), (3e38, 1e-43), (1e30, 1e-38), (3e38, 1e-36), (-2e38, 3e-38)])
+def test_attention_small_scales_and_large_keys(capi, key, scale):
+    """bf16 keys next to the type's end, whose products with a query need more than 32 bits, and scales down to nothing that make logits of them."""
+    g = generator(44)
+    for q_size in (1.0, 100.0):
+        lens, D = [5, 100, 900], 64
+        pages, total = table_for(g, lens, 16)
+        k, v = pool(g, total, 16, 2, D, torch.bfloat16)
+        k.copy_((torch.rand(k.shape, generator=g, device="cuda") * key).to(torch.bfloat16))
+        q, out = randn(g, 3, 4, D) * q_size, torch.empty((3, 4, D), device="cuda")
+        capi.paged_attention_q8_1(q, k, v, pages, i32(lens), scale=scale, out=out, want_q8=False)
+        want, _, far, _ = attended(q, k, v, pages, lens, 16, float(torch.tensor(scale)))
+        assert torch.isfinite(out).all() and ((out.double() - want).abs() <= far).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("Hq,Hk,D,page", [(8, 2, 128, 16), (4, 4, 64, 5), (24, 1, 64, 32), (40, 2, 256, 16), (3, 1, 80, 24)])
 def test_attention_weights(capi, kind, Hq, Hk, D, page):
     check_attention(capi, generator(Hq + D), kind, Hq, Hk, D, page, [1, 0, 15, 700, 64, 2500], weights=True)
