@@ -112,8 +112,10 @@ size_t jq_paged_attention_ws_bytes(int64_t num_rows, int64_t num_q_heads, const 
  * head h goes with key-value head h / (num_q_heads / num_kv_heads).
  *   out = sum_i p_i v_i, p = softmax(scale * q . k_i)
  * A row that sees nothing (length zero or less) gives zeros; a row whose sequence is outside [0, num_seqs) is padding and left as it
- * was in every output.  Lengths beyond max_pages * page_size count as that.  Elements of the cache that a row sees are finite; what
- * lies behind its length or before its window may be anything.  Several rows may see the same sequence (drafted tokens, a short
+ * was in every output.  Lengths beyond max_pages * page_size count as that.  Elements of the cache that a row sees are finite, and with
+ * JQ_KV_BF16 so are its logits and the sum of a column of its values in 32 bits; what
+ * lies behind its length or before its window may be anything.  With JQ_KV_F16 and JQ_KV_E4M3 p_i is rounded to 2^-40 of the row's largest one
+ * where that is more than 2^-23 of itself.  Several rows may see the same sequence (drafted tokens, a short
  * prompt: each with its own length).
  * d_out (fp32 [num_rows][num_q_heads * head_dim]) and d_xq (the Q8_1 blocks of that, for the o-projection, in `order` and `s_mode`;
  * head_dim % 32 == 0 and num_q_heads * head_dim % 128 == 0) are each optional, at least one is required.  The blocks are those that

@@ -9,7 +9,9 @@
 // (16 elements x 8 heads), so the heads are the narrow side and few heads waste little (mma.sync: 8 columns are half of the narrowest
 // tcgen05 tile, and a warp that needs no other one keeps its data in registers between the two products).
 // Queries and probabilities are fp32 and are multiplied as the sum of two fp16 or three bf16 numbers (22 and 24 bits), whose products
-// with a 16-bit element are exact; so nothing is rounded to fewer than 22 bits, and the sums are fp32.
+// with a 16-bit element are exact, and the sums are fp32.  fp16 has few exponents: of a query's elements what is rounded away is up to 2^-24 of
+// their largest, of a probability up to 2^-23 of itself or 2^-40 of the row's largest, whichever is more.  So the n keys of a long row that have
+// next to nothing are together off by n 2^-40 of the largest value at most (a million: 2^-20); the sum of probabilities has them whole.
 //
 // The work is cut into units of 16 keys of one row and key head, all units of the call laid end to end, and every warp takes an equal
 // stretch: long and short rows need no plan on the host, and lengths stay on the device.  A warp needs no other one until its stretch
@@ -94,7 +96,7 @@ struct Parts;  // how an fp32 pair is split into operands whose sum it is
 template <>
 struct Parts<KvF16> {
     static constexpr int N = 2;
-    static constexpr float UP = 16384.f;  // probabilities are held times 2^14: of a million keys as small as 2^-36 nothing is lost
+    static constexpr float UP = 32768.f;  // probabilities, which are 1 at most, are held times 2^15: the most that fp16 has room for
     static constexpr int ROOM = 0, MOST = 100;  // see the queries: a product is below 4 * 2^16 * 256 = 2^26
     static __device__ __forceinline__ void split(float a, float b, uint32_t (&w)[N]) {
         const __half2 h = __floats2half2_rn(a, b);

@@ -478,6 +478,26 @@ def test_attention_logits_of_any_size(capi, kind, size, tokens):
     assert ((weights.double() - gained).abs() <= 20 * U * gained).all()
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,below", [(64, 20.25), (1 << 16, 30.25), (1 << 16, 35.5), (1 << 12, 37.5), (1 << 16, 38.5), (1 << 12, 39.5), (1 << 12, 44.0)])
+def test_attention_keys_that_have_next_to_nothing(capi, kind, n, below):
+    """Of every 32 keys one has nearly all, and a value of nothing; the others have 2^-below of it each, and what is left is theirs."""
+    D, page = 16, 64
+    k, v = (torch.zeros((n // page, page, 1, D), device="cuda") for _ in range(2))
+    k[:, ::32, 0, 0], v[:] = 1.0, 1.0
+    v[:, ::32] = 0.0
+    q = torch.zeros((1, 1, D), device="cuda")
+    q[0, 0, 0] = logit = float(torch.tensor(below * math.log(2)))
+    out = torch.empty_like(q)
+    capi.paged_attention_q8_1(q, k.to(TYPES[kind]), v.to(TYPES[kind]), torch.arange(n // page, dtype=torch.int32, device="cuda")[None], i32([n]), scale=1.0, out=out,
+                              want_q8=False)
+    each = math.exp(-logit)
+    want = 31 * each / (1 + 31 * each)
+    # a share's relative error (see attended(); products of one element: size and widest are the logit); with fp16 parts, the rounding to 2^-40
+    d = (4 * logit + (3 * D / 16 + 2) * 2 * logit + 8 + logit) * U
+    assert ((out.double() - want).abs() <= want * (2 * d + 120 * U) + (0 if kind == "bf16" else 31 * 2.0**-40)).all(), (out[0, 0, 0].item(), want)
+
+
 @pytest.mark.parametrize("key,scale", [(1e38, 0.0), (1e30, 0.0), (3e38, 1e-43), (1e30, 1e-38), (3e38, 1e-36), (-2e38, 3e-38)])
 def test_attention_small_scales_and_large_keys(capi, key, scale):
     """bf16 keys next to the type's end, whose products with a query need more than 32 bits, and scales down to nothing that make logits of them."""
