@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const E
     const int n = tokens_of(a, seq), stays = min(n, a.keep);
     const int thread = part * SELECT_THREADS + threadIdx.x, threads = parts * SELECT_THREADS;
 
-    for (int64_t i = stays + thread; i < a.keep; i += threads) kept[i] = -1;  // (keep is up to 2^31 - 256: a step beyond it needs more bits)
+    for (int behind = a.keep - stays - thread; behind > 0; behind -= threads) kept[a.keep - behind] = -1;  // (a step beyond keep may be beyond 2^31)
     if (n <= a.keep) {  // all stay
         for (int i = thread; i < n; i += threads) {
             kept[i] = i;
