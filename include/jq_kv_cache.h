@@ -145,8 +145,10 @@ int jq_paged_attention_q8_1_device(void *stream, const float *d_q, int64_t q_str
  *   d_new_lens[b]            n (may be d_lens itself)
  *   d_new_weights[b][h]      their weights, and zeros from n up to max_len (may be d_weights; new_weights_stride floats apart)
  * Keys and values move to tokens 0 .. n-1 of the pages in d_new_page_table (num_seqs rows, new_table_stride apart, new_max_pages
- * entries, keep <= new_max_pages * page_size), which are other pages of the same pool; with d_new_page_table NULL they move to the
- * front of the sequence's own pages.  Tokens from n on are left as they were.  Rotated keys stay as they are: their positions do
+ * entries, keep <= new_max_pages * page_size), which are other pages of the same pool, each of one sequence (the cache's own table is
+ * refused); the pages they come from may be shared.  With d_new_page_table NULL they move to the
+ * front of the sequence's own pages, which no other sequence may have: of pages that sequences share for reading, a common start, move
+ * them to new ones.  Tokens from n on are left as they were.  Rotated keys stay as they are: their positions do
  * not change.  max_len is at most jq_kv_evict_max_len() of the current device. */
 int64_t jq_kv_evict_max_len(void);
 int jq_kv_evict_device(void *stream, const jq_kv_cache *cache, const int32_t *d_lens, const float *d_weights, int64_t weights_stride,

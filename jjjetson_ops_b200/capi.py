@@ -354,7 +354,7 @@ def kv_evict(weights: torch.Tensor, lens: torch.Tensor, k_cache: torch.Tensor, v
              kept: Optional[torch.Tensor] = None):
     """Cuts every sequence of the cache down to ``keep`` tokens per key-value head: the first ``sinks``, the last ``recent`` and
     those of the largest ``weights`` ``[sequences, Hkv, tokens]``, in their order.  They move to the pages of ``new_page_table``
-    (other pages of the same pool) or, by default, to the front of their own.  Returns ``(kept, new_lens)``: the tokens' former
+    (other pages of the same pool) or, by default, to the front of their own, which no other sequence may share then.  Returns ``(kept, new_lens)``: the tokens' former
     indices ``[sequences, Hkv, keep]`` (-1 behind the last) and the new lengths.  ``new_weights`` (default: ``weights`` itself)
     receives the kept tokens' weights, then zeros.  ``new_lens`` may be ``lens``."""
     if kept is None:

@@ -370,6 +370,8 @@ int jq_kv_evict_device(void *stream, const jq_kv_cache *cache, const int32_t *d_
     const bool in_place = d_new_page_table == nullptr;
     a.to = a.ix;
     if (!in_place) {
+        if (d_new_page_table == cache->d_page_table)  // rows would be overwritten before they are read
+            return set_error(JQ_ERR_INVALID_ARG, "evict: the new page table is the cache's own; without one tokens stay within their pages");
         if (new_max_pages < 0 || new_max_pages > 0x7FFFFFFF || (keep + cache->page_size - 1) / cache->page_size > new_max_pages)
             return set_error(JQ_ERR_INVALID_ARG, "evict: %lld new pages do not hold %lld tokens", (long long)new_max_pages, (long long)keep);
         if (new_table_stride < new_max_pages && cache->num_seqs > 1)

@@ -847,6 +847,30 @@ def test_evict_bad_pages_and_refusals(capi):
         capi.kv_evict(w, i32([12, 3]), k, v, i32([[0, 1, 2]]), 4)
 
 
+def test_evict_from_pages_that_sequences_share(capi):
+    """Two sequences with a common start: each is cut down into pages of its own, and the shared ones stay as they were."""
+    g = generator(45)
+    k, v = pool(g, 10, 16, 2, 32, torch.float16)
+    k0, v0 = k.clone(), v.clone()
+    pages, target = i32([[4, 1, 7], [4, 1, 9]]), i32([[0, 2], [3, 5]])
+    w = torch.rand((2, 2, 48), generator=g, device="cuda")
+    kept, n = capi.kv_evict(w, i32([48, 40]), k, v, pages, 20, recent=4, new_page_table=target, new_weights=torch.empty_like(w))
+    assert n.tolist() == [20, 20]
+    j = torch.arange(20, device="cuda")
+    for b in range(2):
+        for h in range(2):
+            stay = chosen(w[b, h].tolist(), (48, 40)[b], 20, 4, 0)
+            i = torch.tensor(stay, device="cuda")
+            assert kept[b, h].tolist() == stay
+            for t, t0 in ((k, k0), (v, v0)):
+                assert torch.equal(t[target[b, j // 16].long(), j % 16, h], t0[pages[b, i // 16].long(), i % 16, h])
+    for t, t0 in ((k, k0), (v, v0)):
+        assert torch.equal(t[[1, 4, 6, 7, 8, 9]], t0[[1, 4, 6, 7, 8, 9]])
+    with pytest.raises(capi.JqError) as e:
+        capi.kv_evict(w, i32([48, 40]), k, v, pages, 20, new_page_table=pages)
+    assert e.value.status == capi.ERR_INVALID_ARG
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 def test_evict_budget_next_to_2_31(capi, in_place):
     """The largest budget that is taken: indices one step beyond it have more than 31 bits, and nothing outside the list is written."""

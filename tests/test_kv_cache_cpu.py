@@ -244,6 +244,14 @@ def test_refused_arguments(native_lib, status, call, args):
     assert call(c, c.lib(), **args) == getattr(c, status), c.last_error()
 
 
+def test_eviction_refuses_the_own_table_as_the_new_one(native_lib):
+    """Tokens would move to pages that others are still read from."""
+    c, lib = native_lib, native_lib.lib()
+    own = cache()
+    assert _evict(c, lib, new_table=own.d_page_table, new_pages=4, new_stride=4, descriptor=own) == c.ERR_INVALID_ARG
+    assert "own" in c.last_error()
+
+
 def test_calls_without_rows_need_no_buffers(native_lib):
     """Empty tensors have no address: which of them there are does not matter."""
     c, lib = native_lib, native_lib.lib()
