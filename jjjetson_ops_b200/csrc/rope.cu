@@ -291,6 +291,15 @@ int check_rope(int64_t rows, int64_t heads, int64_t dim, int64_t rotary_dim, flo
     return JQ_OK;
 }
 
+// In the 64 bits of a long double: 53 are a step of 2^-56 turns for a fast pair, which 2^31 positions make 2^-25 turns of.
+uint64_t steps_of(long double radians) {
+    constexpr long double TWO_PI = 6.283185307179586476925286766559L;
+    long double turns = radians / TWO_PI;
+    turns -= floorl(turns);  // whole turns do not count
+    const long double steps = floorl(turns * 18446744073709551616.0L + 0.5L);
+    return steps >= 18446744073709551616.0L ? 0 : (uint64_t)steps;
+}
+
 }  // namespace
 
 int check_kv_cache(const jq_kv_cache *c, KvIndex *ix) {
@@ -345,13 +354,7 @@ int jq_rope_table_from(const double *radians, int64_t n_pairs, uint64_t *table_o
     for (int64_t i = 0; i < n_pairs; ++i) {
         if (!std::isfinite(radians[i])) return set_error(JQ_ERR_INVALID_ARG, "rope table: frequency %lld is not finite", (long long)i);
     }
-    constexpr long double TWO_PI = 6.283185307179586476925286766559L;
-    for (int64_t i = 0; i < n_pairs; ++i) {
-        long double turns = (long double)radians[i] / TWO_PI;
-        turns -= floorl(turns);  // whole turns do not count
-        const long double steps = floorl(turns * 18446744073709551616.0L + 0.5L);
-        table_out[i] = steps >= 18446744073709551616.0L ? 0 : (uint64_t)steps;
-    }
+    for (int64_t i = 0; i < n_pairs; ++i) table_out[i] = steps_of((long double)radians[i]);
     return JQ_OK;
 }
 
@@ -366,28 +369,29 @@ int jq_rope_table(int64_t rotary_dim, double base, int scaling, double factor, i
         return set_error(JQ_ERR_INVALID_ARG, "rope table: factor must be 1 or more");
     if ((scaling == JQ_ROPE_YARN || scaling == JQ_ROPE_WAVELENGTH) && original_length <= 0)
         return set_error(JQ_ERR_INVALID_ARG, "rope table: original_length must be positive");
-    constexpr double PI = 3.14159265358979323846;
-    const double r = (double)rotary_dim;
-    if (scaling == JQ_ROPE_NTK) base *= pow(factor, r / (r > 2 ? r - 2 : 1));
-    if (!std::isfinite(base)) return set_error(JQ_ERR_INVALID_ARG, "rope table: the scaled base is not finite");
-    double radians[512];
-    double low = 0, high = 0;
+    constexpr long double TWO_PI = 6.283185307179586476925286766559L;
+    const long double r = (long double)rotary_dim;
+    long double b = base;
+    if (scaling == JQ_ROPE_NTK) b *= powl(factor, r / (r > 2 ? r - 2 : 1));
+    if (!(b <= 1.7976931348623157e308L)) return set_error(JQ_ERR_INVALID_ARG, "rope table: the scaled base is not finite");
+    long double low = 0, high = 0;
     if (scaling == JQ_ROPE_YARN) {
         // the pair that turns so many times within the original length
-        const auto pair_of = [&](double turns) { return r * log((double)original_length / (turns * 2 * PI)) / (2 * log(base)); };
-        low = fmax(floor(pair_of(32.0)), 0.0);
-        high = fmin(ceil(pair_of(1.0)), r - 1);
+        const auto pair_of = [&](long double turns) { return r * logl((long double)original_length / (turns * TWO_PI)) / (2 * logl(b)); };
+        low = fmaxl(floorl(pair_of(32)), 0);
+        high = fminl(ceill(pair_of(1)), r - 1);
     }
     for (int64_t i = 0; i < rotary_dim / 2; ++i) {
-        double f = pow(base, -2.0 * (double)i / r), divided = 0;  // the share of the pair that is divided by the factor
+        const long double f = powl(b, -2 * (long double)i / r);
+        long double divided = 0;  // the share of the pair that is divided by the factor
         if (scaling == JQ_ROPE_LINEAR) divided = 1;
-        if (scaling == JQ_ROPE_YARN) divided = fmin(fmax(((double)i - low) / fmax(high - low, 0.001), 0.0), 1.0);
-        if (scaling == JQ_ROPE_WAVELENGTH) divided = 1 - fmin(fmax(((double)original_length * f / (2 * PI) - 1.0) / 3.0, 0.0), 1.0);
-        radians[i] = f / factor * divided + f * (1 - divided);
-        if (divided == 0) radians[i] = f;  // (also where there is no factor)
+        if (scaling == JQ_ROPE_YARN) divided = fminl(fmaxl(((long double)i - low) / fmaxl(high - low, 0.001L), 0), 1);
+        if (scaling == JQ_ROPE_WAVELENGTH) divided = 1 - fminl(fmaxl(((long double)original_length * f / TWO_PI - 1) / 3, 0), 1);
+        // (f by itself also where there is no factor)
+        table_out[i] = steps_of(divided == 0 ? f : f / factor * divided + f * (1 - divided));
     }
     *mscale_out = scaling == JQ_ROPE_YARN ? (float)(0.1 * log(factor) + 1.0) : 1.f;
-    return jq_rope_table_from(radians, rotary_dim / 2, table_out);
+    return JQ_OK;
 }
 
 int jq_rope_device(void *stream, const float *d_x, float *d_out, const int32_t *d_positions, const uint64_t *d_table,

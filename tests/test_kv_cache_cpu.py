@@ -147,6 +147,37 @@ def test_scaled_frequencies(native_lib, rotary, how, factor, length):
     assert mscale == pytest.approx(0.1 * math.log(factor) + 1 if how == "yarn" else 1.0, rel=2**-23)
 
 
+@pytest.mark.parametrize("rotary", [2, 20, 128, 1024])
+@pytest.mark.parametrize("base", [10000.0, 500000.0, 1.5])
+@pytest.mark.parametrize("how,factor", [("none", 1.0), ("linear", 3.0), ("ntk", 4.0), ("wavelength", 8.0), ("yarn", 16.0)])
+def test_table_entries_are_rounded_once(native_lib, rotary, base, how, factor):
+    """Against decimal arithmetic: a step, 2^-64 turns, is what the entries are off by, not the step of a frequency in double precision, which
+    2^31 positions make 2^-25 turns of."""
+    pi, length = _pi(), 4096
+    r, b, f0 = Decimal(rotary), Decimal(base), Decimal(factor)
+    if how == "ntk":
+        b *= f0 ** (r / max(r - 2, 1))
+    table, _ = native_lib.rope_table(rotary, base, how, factor, length)
+    if how == "yarn":
+        low, high = ((r * (Decimal(length) / (n * 2 * pi)).ln() / (2 * b.ln())) for n in (32, 1))
+        low, high = max(low.to_integral_value(rounding="ROUND_FLOOR"), Decimal(0)), min(high.to_integral_value(rounding="ROUND_CEILING"), r - 1)
+    for i, got in enumerate(table.tolist()):
+        f = b ** (Decimal(-2 * i) / r)
+        t = Decimal(0)
+        if how == "linear":
+            t = Decimal(1)
+        if how == "yarn":
+            t = min(max((i - low) / max(high - low, Decimal("0.001")), Decimal(0)), Decimal(1))
+        if how == "wavelength":
+            t = 1 - min(max((length * f / (2 * pi) - 1) / 3, Decimal(0)), Decimal(1))
+        f = f / f0 * t + f * (1 - t)
+        # Long doubles have 64 bits, a rounding is 2^-64 of the value: the power's exponent (up to ln(base) of it, with ntk's base some 15), its
+        # base, itself, and less than ten operations (where the wavelength's share counts, it is of numbers up to 4): under 50 roundings, 2^-64 each, of
+        # at most 2^64 / (2 pi) steps: 8; and 1.5 for the fraction (above)
+        error = abs(Decimal(got % 2**64) - f / (2 * pi) * 2**64)
+        assert error <= 10, (i, error)
+
+
 def test_tables_that_are_refused(native_lib):
     c = native_lib
     for args in ((3,), (0,), (-2,), (2048,)):
