@@ -47,11 +47,19 @@ JQ_HOST_DEVICE int32_t kv_length(const KvIndex &ix, int32_t len) {
     return len < 0 ? 0 : len > most ? (int32_t)most : len;
 }
 
-// A turn is 2^64 steps.  `steps` per position times the position, modulo a turn, is exact; the result is in half turns, [-1, 1), and
-// off by 2^-32 from the cut and by half a bit of its own from the conversion.
-JQ_HOST_DEVICE float rope_half_turns(uint64_t steps, int32_t position) {
+// A turn is 2^64 steps.  `steps` per position times the position, modulo a turn, is exact.  The nearest quarter turn is taken off it as
+// an integer; what is left, in half turns, [-1/4, 1/4], is off by 2^-33 from the cut and by half a bit of its own, 2^-27 at most, from the
+// conversion (of a whole half turn it would be 2^-25).
+JQ_HOST_DEVICE float rope_half_turns(uint64_t steps, int32_t position, uint32_t *quarters) {
     const uint64_t angle = steps * (uint64_t)(int64_t)position;
-    return (float)(int32_t)(angle >> 32) * 4.656612873077393e-10f;  // 2^-31
+    *quarters = (uint32_t)((angle + ((uint64_t)1 << 61)) >> 62);
+    return (float)(int32_t)((int64_t)(angle - ((uint64_t)*quarters << 62)) >> 30) * 1.1641532182693481e-10f;  // 2^-33
+}
+// The cosine and sine of an angle from those of what is left without its quarter turns.
+JQ_HOST_DEVICE void rope_add_quarters(uint32_t quarters, float *c, float *s) {
+    const float x = quarters & 1 ? -*s : *c, y = quarters & 1 ? *c : *s;
+    *c = quarters & 2 ? -x : x;
+    *s = quarters & 2 ? -y : y;
 }
 
 }  // namespace jq

@@ -132,7 +132,9 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a) {
     for (int i = threadIdx.x; i < rows * a.half; i += blockDim.x) {
         const int row = i / a.half, pair = i - row * a.half;
         float s, c;
-        sincospif(rope_half_turns(a.table[pair], a.positions[row0 + row]), &s, &c);
+        uint32_t quarters;
+        sincospif(rope_half_turns(a.table[pair], a.positions[row0 + row], &quarters), &s, &c);
+        rope_add_quarters(quarters, &c, &s);
         turn[i] = make_float2(c * a.mscale, s * a.mscale);
     }
     __syncthreads();

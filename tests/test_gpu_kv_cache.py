@@ -144,6 +144,23 @@ def test_rope_strides_and_alignment(capi):
     assert torch.equal(capi.rope(row, positions, table), capi.rope(row.contiguous(), positions, table))
 
 
+def test_rope_sines_of_exact_angles(capi):
+    """Pairs (1, 0): what comes out are cosine and sine themselves, of angles that are exact in integers."""
+    n = 1 << 16
+    g = generator(46)
+    steps = torch.randint(-2**63, 2**63 - 1, (8,), generator=g, device="cuda", dtype=torch.int64)
+    positions = torch.randint(0, 2**24, (n,), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.zeros((n, 1, 16), device="cuda")
+    x[..., :8] = 1.0
+    got = capi.rope(x, positions, steps).double()[:, 0]
+    angle = positions.long()[:, None] * steps  # modulo 2^64, a turn
+    # the angle in 64 bits: its upper 53 bits, to 2^-52 of a turn
+    radians = (angle >> 11).double() * (2 * math.pi / 2.0**53)
+    for part, f in ((got[:, :8], torch.cos), (got[:, 8:], torch.sin)):
+        # what is left of the angle: 2^-27 and 2^-33 half turns, pi of which 0.4 u; sincospif to 2 ulp, which for values up to 1 is 2 u; the products with 1 and 0 are exact
+        assert ((part - f(radians)).abs() <= 2.5 * U).all()
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("T,H,D,R,shift", [(3, 2, 1024, 1024, 1), (2, 3, 1024, 1022, 0), (2, 1, 1022, 1022, 3), (5, 2, 1022, 6, 2), (3, 2, 514, 514, 1),
                                            (700, 3, 514, 258, 0), (1, 2, 1022, 1020, 2), (2, 2, 516, 512, 1)])

@@ -2,6 +2,7 @@
 import ctypes
 import math
 import os
+import random
 import re
 import subprocess
 import sys
@@ -91,6 +92,38 @@ def test_offsets_beyond_32_bits(index):
 def test_lengths_are_cut_to_the_table(index):
     for pages, n, want in ((4, 64, 64), (4, 65, 64), (4, 2**31 - 1, 64), (4, -1, 0), (4, -2**31, 0), (0, 5, 0)):
         assert index([(16, 0, 0, 1, 1, 1, pages, n)])[0][2] == want
+
+
+def test_angles_are_a_quarter_turn_and_a_rest(tmp_path):
+    """csrc/kv_index.h compiled for the host: the rest is the exact one to 2^-33 and half a bit, and quarter turns change what sine and cosine are."""
+    (tmp_path / "x.cpp").write_text("""
+#include <cstdio>
+#include "kv_index.h"
+int main() {
+    unsigned long long steps; int position;
+    while (scanf("%llu %d", &steps, &position) == 2) {
+        uint32_t quarters;
+        const float rest = jq::rope_half_turns(steps, position, &quarters);
+        float c = 3, s = 5;
+        jq::rope_add_quarters(quarters, &c, &s);
+        printf("%u %.17g %g %g\\n", quarters, (double)rest, c, s);
+    }
+}
+""")
+    exe = str(tmp_path / "x")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "jjjetson_ops_b200", "csrc"), str(tmp_path / "x.cpp"), "-o", exe], check=True)
+    rng = random.Random(5)
+    cases = [(s, p) for s in (0, 1, 2**61 - 1, 2**61, 2**61 + 1, 2**62, 2**63 - 1, 2**63, 2**64 - 2**61, 2**64 - 2**61 - 1, 2**64 - 1)
+             for p in (0, 1, -1, 2, 3, -3, 2**31 - 1, -2**31)]
+    cases += [(rng.getrandbits(64), rng.randrange(-2**31, 2**31)) for _ in range(2000)]
+    out = subprocess.run([exe], input="\n".join("%d %d" % c for c in cases), capture_output=True, text=True, check=True).stdout.split()
+    for i, (steps, position) in enumerate(cases):
+        quarters, rest, c, s = int(out[4 * i]), float(out[4 * i + 1]), float(out[4 * i + 2]), float(out[4 * i + 3])
+        exact = Decimal(steps * position % 2**64) / 2**63 - Decimal(quarters) / 2  # in half turns
+        exact = exact - 2 if exact > 1 else exact
+        assert abs(exact) <= Decimal("0.25") and abs(rest) <= 0.25 and quarters in (0, 1, 2, 3), (steps, position)
+        assert abs(Decimal(rest) - exact) <= Decimal(2) ** -33 + abs(exact) * Decimal(2) ** -24, (steps, position)
+        assert (c, s) == ((3, 5), (-5, 3), (-3, -5), (5, -3))[quarters]  # times i for every quarter turn
 
 
 # ---- rotary tables ------------------------------------------------------------------------------------------------
