@@ -429,6 +429,26 @@ def test_attention_pages_and_strides(capi, kind, page, layout):
     check_attention(capi, generator(page), kind, 8, 2, 64, page, [70, 1, 300, 2, 511], layout)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [32, 144, 160, 176, 208, 224, 240])
+def test_attention_heads_between_the_instances(capi, kind, D):
+    """Widths that fill their instance's tiles in part."""
+    check_attention(capi, generator(D), kind, 4, 2, D, 16, [1, 40, 333])
+    check_attention(capi, generator(D), kind, 24, 2, D, 5, [1, 40, 333], weights=True)
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_attention_lengths_beyond_the_table(capi, window):
+    """They count as what the row of the table has room for; negative ones as nothing."""
+    g = generator(48)
+    k, v = pool(g, 4, 16, 2, 64, torch.float16)
+    pages, q = i32([[3, 0], [1, 2], [0, 1]]), randn(g, 3, 4, 64)
+    cut, beyond = torch.empty_like(q), torch.empty_like(q)
+    capi.paged_attention_q8_1(q, k, v, pages, i32([32, 32, 0]), window=window, out=cut, want_q8=False)
+    capi.paged_attention_q8_1(q, k, v, pages, i32([33, 2**31 - 1, -2**31]), window=window, out=beyond, want_q8=False)
+    assert torch.equal(cut, beyond) and (beyond[2] == 0).all()
+
+
 @pytest.mark.parametrize("rows,length,Hq,Hk", [(1, 1, 4, 4), (1, 40, 4, 1), (1, 3000, 8, 1), (1, 20011, 4, 2), (3, 5000, 8, 8), (40, 90, 8, 8), (200, 33, 4, 4),
                                                (33, 700, 16, 16), (600, 5, 2, 1), (5, 9000, 32, 2)])
 @pytest.mark.parametrize("kind", ["f16", "bf16", "e4m3"])
@@ -837,6 +857,12 @@ def test_evict_lengths_and_weights_in_place(capi):
     check_evict(capi, g, "f16", 2, 64, 16, [500, 30, 100], 512, 100, 10, 4, in_place=True, same_weights=False)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_lengths_beyond_the_weights(capi, in_place):
+    """They count as the weights' length."""
+    check_evict(capi, generator(28), "f16", 2, 64, 16, [400, 33, 2**31 - 1], 300, 100, 9, 3, in_place=in_place)
+
+
 def test_evict_many_sequences_and_a_long_one(capi):
     check_evict(capi, generator(24), "bf16", 2, 16, 16, [int(n) for n in np.random.default_rng(1).integers(0, 80, 300)], 80, 24, 5, 1)
     check_evict(capi, generator(25), "f16", 1, 16, 64, [300001], 300001, 5000, 100, 4)
@@ -912,6 +938,58 @@ def test_evict_budget_next_to_2_31(capi, in_place):
         for old, new, slots in ((5, 6, 16), (0, 2, 16), (3, 1, 8)):
             k0[new, :slots], v0[new, :slots] = k0[old, :slots], v0[old, :slots]
     assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_and_evict_in_graphs_and_on_two_streams(capi, in_place):
+    """Recorded and replayed on two streams at once, on caches of their own, with inputs that change in between: the bits of eager calls."""
+    g = generator(47)
+    B, Hq, Hk, D, page, S, keep = 3, 4, 2, 64, 16, 3000, 700
+    table, _ = capi.rope_table(D, device="cuda")
+    sides = []
+    for i in range(2):
+        pages, total = table_for(g, [S] * B, page, spare=0)
+        new_pages, more = table_for(g, [keep] * B, page, spare=0)
+        k, v = pool(g, total + more, page, Hk, D, torch.float16)
+        side = dict(pages=pages, new=None if in_place else new_pages + total, k=k, v=v, w=torch.zeros((B, Hk, S), device="cuda"), lens=i32([0] * B), at=i32([0] * B),
+                    qkv=torch.zeros((B, (Hq + 2 * Hk) * D), device="cuda"), q=torch.zeros((B, Hq, D), device="cuda"), kept=i32([[[0] * keep] * Hk] * B),
+                    stream=torch.cuda.Stream())
+        sides.append(side)
+
+    def step(s):
+        capi.rope_append(s["qkv"], s["at"], table, s["k"], s["v"], s["pages"], s["at"], q_out=s["q"])
+        capi.kv_evict(s["w"], s["lens"], s["k"], s["v"], s["pages"], keep, recent=50, sinks=4, new_page_table=s["new"], new_lens=s["lens"], kept=s["kept"])
+
+    fields = ("k", "v", "w", "lens", "q", "kept")
+    for s in sides:
+        with torch.cuda.stream(s["stream"]):
+            s["stream"].wait_stream(torch.cuda.default_stream())
+            step(s)
+            s["stream"].synchronize()
+            s["graph"] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(s["graph"], stream=s["stream"]):
+                step(s)
+    for lens in ([3000, 701, 5], [700, 0, 2999], [1500, 1501, 1]):
+        expected = []
+        for s in sides:
+            s["qkv"].copy_(randn(g, *s["qkv"].shape))
+            s["w"].copy_(torch.rand(s["w"].shape, generator=g, device="cuda"))
+            s["lens"].copy_(i32(lens))
+            s["at"].copy_((i32(lens) - 1).clamp(min=0))
+            before = {f: s[f].clone() for f in fields}
+            step(s)
+            expected.append({f: s[f].clone() for f in fields})
+            for f in fields:
+                s[f].copy_(before[f])
+        torch.cuda.synchronize()
+        for s in sides:
+            with torch.cuda.stream(s["stream"]):
+                s["graph"].replay()
+        torch.cuda.synchronize()
+        for s, want in zip(sides, expected):
+            assert s["lens"].tolist() == [min(n, keep) for n in lens]
+            for f in fields:
+                assert torch.equal(s[f], want[f]), f
 
 
 # ---- all of it, the way a decoder uses it --------------------------------------------------------------------------------------
