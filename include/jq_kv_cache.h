@@ -39,8 +39,8 @@ typedef enum jq_kv_type {
  * page * stride_page + slot * stride_slot + h * stride_head of d_k and of d_v, and are contiguous.  Any order of the three
  * strides will do.  A page belongs to one sequence (sequences that share the pages of a common start may read them).
  *
- * A page number outside [0, num_pages) is never followed: tokens there are neither written nor attended to, and the fault word
- * of jq_device_fault() is set to 4 if a kernel needed one.  Entries behind a sequence's last page are not looked at. */
+ * A page number outside [0, num_pages) is never followed: tokens there are neither written nor attended to, and
+ * jq_device_fault() reports 4 if a kernel needed one.  Entries behind a sequence's last page are not looked at. */
 typedef struct jq_kv_cache {
     void *d_k;                /* 16-byte aligned, as are all rows: strides in bytes are multiples of 16 */
     void *d_v;
@@ -103,7 +103,8 @@ int jq_rope_kv_append_device(void *stream, const float *d_qkv, int64_t qkv_strid
 
 /* ---- attention ---------------------------------------------------------------------------------------- */
 
-/* Bytes of workspace for jq_paged_attention_q8_1_device, whatever the lengths are; with `weights` for calls that accumulate weights.
+/* Bytes of workspace for jq_paged_attention_q8_1_device, whatever the lengths are; with `weights` for calls that accumulate weights
+ * (4 bytes more for every row, query head and token that the page table has room for).
  * The size depends on the current device.  0 after an error. */
 size_t jq_paged_attention_ws_bytes(int64_t num_rows, int64_t num_q_heads, const jq_kv_cache *cache, int weights);
 

@@ -13,7 +13,7 @@ namespace jq {
 constexpr int FAULT_BAD_PAGE = 4;
 constexpr int64_t KV_MAX_DIM = 256;
 
-// Checks the descriptor and fills the kernels' indices.  `write`: the cache is written.
+// Checks the descriptor and fills the kernels' indices.
 int check_kv_cache(const jq_kv_cache *c, KvIndex *ix);
 
 inline int kv_element_bytes(int type) { return type == JQ_KV_E4M3 ? 1 : 2; }

@@ -58,7 +58,9 @@ struct Counts {
 };
 
 // (two blocks on an SM, which leaves 32 registers and spills one: with one block, of 38, 128 blocks in clusters of eight take turns.  A whole
-// call, us with one / two: 17 x 4 heads of 27173 69.7 / 55.3, 2 x 8 of 20000 41.0 / 34.8, 6 x 8 of 9000 34.8 / 28.7; 8 of 100003 53.3 both)
+// call into other pages, its data not in L2, us with one / two: 17 x 4 heads of 27173 down to 2000 70.7 / 56.4, down to 8000 142 / 130, 2 x 8 of 20000
+// to 4000 48.2 / 42.0, 6 x 8 of 9000 to 2000 48.1 / 42.0, 24 x 8 of 5000 to 1000 58.4 / 56.4; 8 of 100003 to 16000 54.3 both.  21 x 8 of 3000
+// to 1000 within their pages lose: 37.9 / 42.0)
 __global__ void __launch_bounds__(SELECT_THREADS, 2) evict_select_kernel(const EvictArgs a) {
     extern __shared__ __align__(16) float w[];  // this block's slice
     __shared__ __align__(16) uint32_t bins[DIGITS][BINS];
@@ -387,7 +389,8 @@ int jq_kv_evict_device(void *stream, const jq_kv_cache *cache, const int32_t *d_
     a.row_bytes = (int)cache->head_dim * kv_element_bytes(cache->type);
     a.fault = device_fault_ptr();
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Blocks per head: one for every 2048 weights, but no more than run at a time (two on an SM), as far as shared memory allows.
+    // Blocks per head: one for every 2048 weights, but no more than two for an SM, and as many as it takes for a slice to fit (two slices of up to
+    // some 22 000 weights fit on an SM; blocks with longer ones wait for one another where there are more than SMs)
     DeviceCaps caps;
     if (int rc = device_caps(&caps)) return rc;
     const int64_t heads = a.kv_heads * cache->num_seqs;
